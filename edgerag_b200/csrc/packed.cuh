@@ -1,0 +1,96 @@
+// What the kernels of attention_packed.cu and attention_packed_tc.cu share: the description of a call, the rows a block owns, and which
+// keys each of them sees.
+//
+// Rows.  The query heads that share a kv head are neighbours, so the rows of one kv head are (token, head in the group) pairs, row r being
+// token r / G, head kvh * G + r % G (G = query heads per kv head).  A block owns a run of such rows; every key it fetches serves them all.
+//
+// Three kinds of calls:
+//   kPrompt   keys lie in rows beside the queries, a sequence's rows one behind the other; row i of a sequence sees its keys 0..i
+//   kPrefix   keys are the first `prefix_len` of every sequence and lie in the pages `prefix_pages`; a block's rows are of all sequences
+//   kOwn      keys are those of one sequence from `prefix_len` on and lie in the sequence's own pages
+// In the last two a row sees the keys up to its token's position.
+//
+// The softmax runs in powers of two: scores are scaled by scale * log2(e).  A call whose keys are cut into pieces leaves a record for each
+// (token, head, piece): D floats of sum_j 2^(s_j - m) v_j, and (m, sum_j 2^(s_j - m)); a record whose sum is 0 has no values.
+// attention_merge_kernel joins the records of a row.
+#pragma once
+
+#include "common.cuh"
+
+namespace erb {
+
+constexpr int kPrompt = 0, kPrefix = 1, kOwn = 2;
+
+// Codes of the status word beside those of waits: a page that lies outside the pool, sequences that do not lie inside the rows.
+constexpr int kBadPage = 9000001, kBadStarts = 9000002;
+
+struct PackedArgs {
+  const elem_t* q;
+  elem_t* out;
+  const elem_t *k, *v;             // kPrompt: rows; else the pools [n_pages][nkv][page_size][D]
+  long long ld_q, ld_out, ld_k, ld_v;
+  int n_pages, page_size;
+  const int* tables;               // kOwn: [n_seqs][table_ld]
+  int table_ld;
+  const int* prefix_pages;
+  int prefix_len;
+  const int* seq_starts;
+  const int* positions;
+  int n_seqs, n_tokens, nq, nkv, D;
+  float scale_log2;
+  float *part_o, *part_ml;         // records: [(token * nq + head) * n_rec + piece]
+  int n_rec, rec0, pieces;         // records of a row, the first of this call's pieces, how many pieces it cuts the keys into
+  int piece_keys;                  // kOwn: keys of a piece (the last one takes the rest)
+  int* status;
+};
+
+__device__ __forceinline__ void report(int* status, int code) { atomicCAS(status, 0, code); }
+
+// The sequence and the row tile of block `index` among the tiles of `rows` rows that the sequences give, one after the other; the whole
+// warp asks.  seq < 0: there is no such tile.
+__device__ __forceinline__ void find_tile(const int* __restrict__ seq_starts, int n_seqs, int G, int rows, int index, int& seq, int& tile) {
+  const int lane = threadIdx.x & 31;
+  seq = -1;
+  tile = 0;
+  for (int s0 = 0; s0 < n_seqs; s0 += 32) {
+    const int s = s0 + lane;
+    const int len = s < n_seqs ? max(0, seq_starts[s + 1] - seq_starts[s]) : 0;
+    const int mine = (int)(((long long)len * G + rows - 1) / rows);
+    int upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int before = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += before;
+    }
+    const unsigned here = __ballot_sync(0xffffffffu, index >= upto - mine && index < upto);
+    if (here) {
+      const int who = __ffs(here) - 1;
+      seq = s0 + who;
+      tile = index - __shfl_sync(0xffffffffu, upto - mine, who);
+      return;
+    }
+    index -= __shfl_sync(0xffffffffu, upto, 31);
+  }
+}
+
+// Where key `key` of this block lies: its row for the head `kvh` (rows of D entries in a pool, of ld entries for kPrompt), or null for a
+// page that is none of the pool's (reported).
+template <int MODE>
+__device__ __forceinline__ void key_rows(const PackedArgs& a, const int* table, long long first_row, int kvh, int key, const elem_t*& k, const elem_t*& v) {
+  if (MODE == kPrompt) {
+    k = a.k + (first_row + key) * a.ld_k + (long long)kvh * a.D;
+    v = a.v + (first_row + key) * a.ld_v + (long long)kvh * a.D;
+  } else {
+    const int page = table[key / a.page_size];
+    if (page < 0 || page >= a.n_pages) {
+      report(a.status, kBadPage);
+      k = v = nullptr;
+      return;
+    }
+    const long long row = (((long long)page * a.nkv + kvh) * a.page_size + key % a.page_size) * a.D;
+    k = a.k + row;
+    v = a.v + row;
+  }
+}
+
+}  // namespace erb

@@ -9,7 +9,10 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import math
 from ctypes import c_float, c_int, c_longlong, c_void_p
+from fractions import Fraction
+from typing import NamedTuple
 
 import torch
 
@@ -143,6 +146,14 @@ _SIGNATURES = {
                           c_void_p, c_void_p],
     "erb_moe_product": [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int,
                         c_int, c_int, c_void_p, c_void_p, c_void_p],
+    "erb_rotary_append": [c_void_p, c_void_p, c_longlong, c_longlong, c_void_p, c_void_p, c_longlong, c_longlong, c_void_p, c_longlong,
+                          c_void_p, c_void_p, c_float, c_float, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int,
+                          c_int, c_int, c_int, c_int, c_void_p, c_void_p],
+    "erb_attention_prompt": [c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_int, c_int, c_void_p, c_longlong,
+                             c_int, c_int, c_int, c_float, c_void_p, c_void_p],
+    "erb_attention_shared_prefix": [c_void_p, c_longlong, c_void_p, c_void_p, c_int, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p,
+                                    c_void_p, c_int, c_int, c_void_p, c_longlong, c_int, c_int, c_int, c_float, c_int, c_int, c_int,
+                                    c_void_p, c_void_p, c_void_p, c_void_p],
     "erb_sample_rows": [c_void_p, c_longlong, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p],
 }
 
@@ -2263,6 +2274,235 @@ def attention_prefill_tc(qkv: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
           *_gate(gate, out, n_q_heads * d), _stream())
     if key_splits > 1:
         launch_counts["own"] += 1          # the merge of the ranges
+
+
+# --- requests' rows from their projections to their attention ----------------------------------
+
+def _packed_rows(t: torch.Tensor, name: str, who: str, rows: int, width: int, dtype: torch.dtype, written: bool = False) -> int:
+    """Checks rows of heads (inner stride 1, any stride between rows); their stride."""
+    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != width or t.dtype != dtype:
+        raise KernelError(f"{who}: {name} must be [{rows}, {width}] of {dtype}, got {list(t.shape)} of {t.dtype}")
+    if (width > 1 and t.stride(1) != 1) or (written and rows > 1 and t.stride(0) < width):
+        raise KernelError(f"{who}: rows of {name} must be contiguous" + (" and may not overlap" if written else ""))
+    return t.stride(0) if rows > 1 else width
+
+
+def _packed_vector(t: torch.Tensor | None, name: str, who: str, dtype: torch.dtype, at_least: int) -> None:
+    if t is None or t.dtype != dtype or t.numel() < at_least or not t.is_contiguous():
+        raise KernelError(f"{who}: {name} must be contiguous {dtype} with at least {at_least} entries")
+
+
+def _on_this_device(who: str, **tensors) -> None:
+    """Every tensor on the current CUDA device: that is where the launch goes."""
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        _need(t, name, contiguous=False)
+        if t.get_device() != torch._C._cuda_getDevice():
+            raise KernelError(f"{who}: {name} is on {t.device}, the current device is cuda:{torch._C._cuda_getDevice()}")
+
+
+_INVERSE_TURN = Fraction("0.159154943091895335768883763372514362034459645740456448747667344")       # 1 / (2 pi)
+
+
+def rotary_turns(frequencies: torch.Tensor) -> torch.Tensor:
+    """Frequencies (radians per position, float64) as ``rotary_append`` takes them: turns per position in units of 2^-64 turn, modulo a
+    turn, int64 on the CPU.  Positions times these, modulo 2^64, are angles without the rounding that a product of floats has far out."""
+    if not torch.isfinite(frequencies).all():
+        raise KernelError("rotary_turns: a frequency is not finite")
+    units = [math.floor(Fraction(f) * _INVERSE_TURN * 2**64) % 2**64 for f in frequencies.double().reshape(-1).tolist()]
+    return torch.tensor([u - 2**64 if u >= 2**63 else u for u in units], dtype=torch.int64)
+
+
+def rotary_append(q: torch.Tensor, positions: torch.Tensor, turns: torch.Tensor | None, n_q_heads: int, n_kv_heads: int, head_dim: int, *,
+                  k: torch.Tensor | None = None, v: torch.Tensor | None = None, pairs: bool = False, multiplier: float = 1.0,
+                  q_norm: torch.Tensor | None = None, k_norm: torch.Tensor | None = None, eps: float = 0.0,
+                  q_out: torch.Tensor | None = None, k_out: torch.Tensor | None = None, slots: torch.Tensor | None = None,
+                  k_pages: torch.Tensor | None = None, v_pages: torch.Tensor | None = None, status: torch.Tensor | None = None) -> None:
+    """Queries and keys made ready for attention in one pass, keys and values appended to the cache on the way.
+
+    ``q`` ``[tokens, n_q_heads * head_dim]``, ``k`` and ``v`` ``[tokens, n_kv_heads * head_dim]``: rows with any stride between them (views
+    of one projection's rows, say).  Per head, in float with one rounding at the end: unit RMS times ``q_norm`` / ``k_norm`` (where given,
+    float32 ``[head_dim]``; ``eps``), then the first ``2 * len(turns)`` entries turned by the token's position: entries ``(i, i + len(turns))``
+    or, with ``pairs``, ``(2 i, 2 i + 1)``, cosine and sine times ``multiplier``.  ``turns`` (``rotary_turns`` of the scaled frequencies, on the
+    device; None: nothing is turned) makes the angles right at any position of int32.
+
+    Queries go to ``q_out`` (None: in place).  With ``k_pages`` and ``v_pages`` ``[pages, n_kv_heads, page_size, head_dim]``, keys and values (as
+    they are) go to slot ``slots[token]`` (int32, ``page * page_size + offset``, no two alike; negative: nowhere), and keys to ``k_out`` only if it
+    is given; without pages keys go to ``k_out`` (None: in place) and there is no ``v``.  A slot behind the pool is left alone and sets
+    ``status`` (int32) to the token's number plus one."""
+    who = "rotary_append"
+    if q.dtype not in _ELEM or q.dim() != 2:
+        raise KernelError(f"{who}: q must be rows of float32 or bfloat16")
+    if n_q_heads <= 0 or n_kv_heads < 0 or not 0 < head_dim <= 1024:
+        raise KernelError(f"{who}: heads {n_q_heads} / {n_kv_heads} of {head_dim} (at most 1024)")
+    n, kw = q.shape[0], n_kv_heads * head_dim
+    ld_q = _packed_rows(q, "q", who, n, n_q_heads * head_dim, q.dtype, written=q_out is None)
+    ld_qo = ld_q if q_out is None else _packed_rows(q_out, "q_out", who, n, n_q_heads * head_dim, q.dtype, written=True)
+    ld_k = ld_ko = ld_v = kw
+    paged = k_pages is not None or v_pages is not None
+    if k is None and (v is not None or k_out is not None or paged or k_norm is not None):
+        raise KernelError(f"{who}: k_out, k_norm, values and pages need keys")
+    if (v is not None) != paged:
+        raise KernelError(f"{who}: values go to pages: v, k_pages and v_pages come together")
+    if k is not None:
+        if n_kv_heads <= 0:
+            raise KernelError(f"{who}: keys need n_kv_heads")
+        ld_k = _packed_rows(k, "k", who, n, kw, q.dtype, written=k_out is None and not paged)
+        ld_ko = ld_k
+        if k_out is not None:
+            ld_ko = _packed_rows(k_out, "k_out", who, n, kw, q.dtype, written=True)
+    if n:
+        _packed_vector(positions, "positions", who, torch.int32, n)
+    rot = 0
+    if turns is not None:
+        _packed_vector(turns, "turns", who, torch.int64, 0)
+        rot = 2 * turns.numel()
+        if rot > head_dim:
+            raise KernelError(f"{who}: {turns.numel()} pairs do not fit into heads of {head_dim}")
+    for name, w in (("q_norm", q_norm), ("k_norm", k_norm)):
+        if w is not None:
+            _packed_vector(w, name, who, torch.float32, head_dim)
+    n_pages = page_size = 0
+    if paged:
+        if k_pages is None or v_pages is None or k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.dtype != q.dtype or v_pages.dtype != q.dtype:
+            raise KernelError(f"{who}: k_pages and v_pages must be two pools of one shape and of q's type")
+        n_pages, heads, page_size, width = k_pages.shape
+        if heads != n_kv_heads or width != head_dim or not k_pages.is_contiguous() or not v_pages.is_contiguous():
+            raise KernelError(f"{who}: page layout is not contiguous [pages, kv heads, page_size, head_dim]")
+        if n_pages * page_size == 0:
+            raise KernelError(f"{who}: the pool has no page")
+        ld_v = _packed_rows(v, "v", who, n, kw, q.dtype)
+        if n:
+            _packed_vector(slots, "slots", who, torch.int32, n)
+        _packed_vector(status, "status", who, torch.int32, 1)
+    _on_this_device(who, q=q, q_out=q_out, k=k, k_out=k_out, v=v, positions=positions, turns=turns, q_norm=q_norm, k_norm=k_norm, slots=slots,
+                    k_pages=k_pages, v_pages=v_pages, status=status)
+    if n == 0:
+        return
+    _call(_fn("rotary", _elem(q), "erb_rotary_append"), q, q if q_out is None else q_out, ld_q, ld_qo, k,
+          (None if paged else k) if k_out is None else k_out, ld_k, ld_ko, v, ld_v, q_norm, k_norm, float(eps), float(multiplier), positions,
+          turns, rot, int(bool(pairs)), slots if paged else None, k_pages, v_pages, n_pages, page_size, n, n_q_heads, n_kv_heads, head_dim, status, _stream())
+
+
+def _grouped_heads(who: str, n_q_heads: int, n_kv_heads: int, head_dim: int, scale: float) -> None:
+    if n_q_heads <= 0 or n_kv_heads <= 0 or n_q_heads % n_kv_heads:
+        raise KernelError(f"{who}: {n_q_heads} query heads cannot share {n_kv_heads} kv heads evenly")
+    if not 0 < head_dim <= 256:
+        raise KernelError(f"{who}: head size {head_dim} (at most 256)")
+    if not (math.isfinite(scale) and scale > 0):
+        raise KernelError(f"{who}: scale {scale} must be positive")
+
+
+def attention_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seq_starts: torch.Tensor, out: torch.Tensor, n_q_heads: int,
+                     n_kv_heads: int, scale: float, status: torch.Tensor) -> None:
+    """Causal attention over whole prompts, packed one behind the other; keys and values lie in rows, not in the cache.
+
+    ``q`` and ``out`` ``[tokens, n_q_heads * head_dim]``, ``k`` and ``v`` ``[tokens, n_kv_heads * head_dim]`` (rows with any stride between them:
+    views of one projection's rows); ``seq_starts`` int32 ``[n + 1]``, ascending: sequence ``s`` is rows ``seq_starts[s]`` to ``seq_starts[s + 1]``,
+    possibly none.  Row ``i`` of a sequence sees its rows ``0 .. i``; query head ``h`` reads kv head ``h // (n_q_heads // n_kv_heads)``.  Rows outside
+    the sequences are left as they are.  Starts outside the rows set ``status`` (int32)."""
+    who = "attention_prompt"
+    if q.dtype not in _ELEM or q.dim() != 2:
+        raise KernelError(f"{who}: q must be rows of float32 or bfloat16")
+    n, head_dim = q.shape[0], q.shape[1] // max(n_q_heads, 1)
+    _grouped_heads(who, n_q_heads, n_kv_heads, head_dim, scale)
+    ld_q = _packed_rows(q, "q", who, n, n_q_heads * head_dim, q.dtype)
+    ld_k = _packed_rows(k, "k", who, n, n_kv_heads * head_dim, q.dtype)
+    ld_v = _packed_rows(v, "v", who, n, n_kv_heads * head_dim, q.dtype)
+    ld_o = _packed_rows(out, "out", who, n, n_q_heads * head_dim, q.dtype, written=True)
+    _packed_vector(seq_starts, "seq_starts", who, torch.int32, 1)
+    _packed_vector(status, "status", who, torch.int32, 1)
+    if n * (n_q_heads // n_kv_heads) >= 1 << 30:
+        raise KernelError(f"{who}: {n} tokens of {n_q_heads} heads in one call")
+    _on_this_device(who, q=q, k=k, v=v, seq_starts=seq_starts, out=out, status=status)
+    if n == 0 or seq_starts.numel() == 1:
+        return
+    _call(_fn("attention_packed", _elem(q), "erb_attention_prompt"), q, ld_q, k, ld_k, v, ld_v, seq_starts, seq_starts.numel() - 1, n, out, ld_o,
+          n_q_heads, n_kv_heads, head_dim, float(scale), status, _stream())
+
+
+class SharedPrefixPlan(NamedTuple):
+    """How ``attention_shared_prefix`` cuts a batch's keys into pieces (``shared_prefix_plan``)."""
+
+    prefix_pieces: int       # blocks that share the prefix's keys
+    own_pieces: int          # pieces of a request's own keys, of ``piece_keys`` each (the last takes the rest)
+    piece_keys: int
+    floats: int              # float32 entries of scratch
+
+
+def shared_prefix_plan(n_tokens: int, n_seqs: int, n_q_heads: int, n_kv_heads: int, head_dim: int, dtype: torch.dtype, page_size: int,
+                       prefix_len: int, max_keys: int, max_tokens: int = 1, sms: int | None = None) -> SharedPrefixPlan:
+    """The plan for a batch of ``n_tokens`` rows of ``n_seqs`` requests: ``max_keys`` bounds the longest context, ``max_tokens`` a request's rows in
+    the call.  Both only size the launch: a longer request is slower, not wrong.  ``sms``: multiprocessors (None: the current device's)."""
+    _grouped_heads("shared_prefix_plan", n_q_heads, n_kv_heads, head_dim, 1.0)
+    if min(n_tokens, n_seqs, prefix_len) < 0 or page_size <= 0:
+        raise KernelError("shared_prefix_plan: negative sizes")
+    sms = _sms(torch.device("cuda", torch._C._cuda_getDevice())) if sms is None else sms
+    own_keys = max(1, max_keys - prefix_len)
+    # Two blocks a multiprocessor, tiles of 64 keys, two tiles a piece at least.
+    rows = n_tokens * (n_q_heads // n_kv_heads)
+    blocks = max(1, -(-rows // 64) * n_kv_heads)
+    tiles = -(-prefix_len // 64)
+    prefix_pieces = min(max(1, 2 * sms // blocks), max(1, tiles // 2), 64) if prefix_len else 0
+    own_pieces = min(max(1, 2 * sms // max(1, n_seqs * n_kv_heads)), max(1, own_keys // 128), 64)
+    piece_keys = -(-own_keys // (64 * own_pieces)) * 64
+    own_pieces = -(-own_keys // piece_keys)
+    records = prefix_pieces + own_pieces
+    floats = n_tokens * n_q_heads * records * (head_dim + 2) if records > 1 else 0
+    return SharedPrefixPlan(prefix_pieces, own_pieces, piece_keys, floats)
+
+
+def attention_shared_prefix(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, prefix_pages: torch.Tensor, prefix_len: int,
+                            block_tables: torch.Tensor, seq_starts: torch.Tensor, positions: torch.Tensor, out: torch.Tensor, n_q_heads: int,
+                            scale: float, plan: SharedPrefixPlan, scratch: torch.Tensor, status: torch.Tensor) -> None:
+    """Attention of a batch whose requests share their first ``prefix_len`` keys: those are read once for all rows, each request's own after
+    them, and the two are joined by the softmax's maxima and sums.
+
+    ``q`` and ``out`` ``[tokens, n_q_heads * head_dim]`` (any stride between rows); request ``s`` has the rows ``seq_starts[s]`` to
+    ``seq_starts[s + 1]`` (int32, ascending; one row each in a decode step, several where new tokens come together, none at all), row ``t`` at
+    position ``positions[t]`` (int32) of its request: it sees the keys ``0 .. positions[t]``.  Pools ``[pages, kv heads, page_size, head_dim]``;
+    ``prefix_pages`` (int32): the pages of keys ``0 .. prefix_len - 1``; ``block_tables`` int32 ``[requests, entries]``: entry ``i`` is the page of
+    a request's keys ``i * page_size ..`` (entries of pages wholly inside the prefix are not read; the page that the prefix ends in has a copy of
+    the request's own).  ``plan`` is ``shared_prefix_plan``'s for these sizes, ``scratch`` float32 with ``plan.floats`` entries.  Rows outside the
+    requests are left as they are, a row that sees no key becomes zeros.  A page number outside the pool, a position behind the table or starts
+    outside the rows set ``status`` (int32); the results are then not valid."""
+    who = "attention_shared_prefix"
+    if q.dtype not in _ELEM or q.dim() != 2 or k_pages.dim() != 4:
+        raise KernelError(f"{who}: q must be rows of float32 or bfloat16, pools [pages, kv heads, page_size, head_dim]")
+    n = q.shape[0]
+    n_pages, n_kv_heads, page_size, head_dim = k_pages.shape
+    _grouped_heads(who, n_q_heads, n_kv_heads, head_dim, scale)
+    ld_q = _packed_rows(q, "q", who, n, n_q_heads * head_dim, q.dtype)
+    ld_o = _packed_rows(out, "out", who, n, n_q_heads * head_dim, q.dtype, written=True)
+    if k_pages.shape != v_pages.shape or k_pages.dtype != q.dtype or v_pages.dtype != q.dtype or not k_pages.is_contiguous() or not v_pages.is_contiguous() \
+            or n_pages * page_size == 0:
+        raise KernelError(f"{who}: pools must be contiguous, of one shape and of q's type")
+    if prefix_len < 0 or prefix_len > 0x7fffffff - page_size:
+        raise KernelError(f"{who}: prefix of {prefix_len} keys")
+    _packed_vector(prefix_pages, "prefix_pages", who, torch.int32, -(-prefix_len // page_size))
+    _packed_vector(seq_starts, "seq_starts", who, torch.int32, 1)
+    n_seqs = seq_starts.numel() - 1
+    if block_tables.dim() != 2 or block_tables.dtype != torch.int32 or block_tables.shape[0] < n_seqs or block_tables.shape[1] < 1 or not block_tables.is_contiguous():
+        raise KernelError(f"{who}: block_tables must be contiguous int32 [requests, entries]")
+    _packed_vector(positions, "positions", who, torch.int32, n)
+    _packed_vector(status, "status", who, torch.int32, 1)
+    if n * (n_q_heads // n_kv_heads) >= 1 << 30 or n_seqs >= 1 << 24:
+        raise KernelError(f"{who}: {n} tokens of {n_q_heads} heads in one call")
+    records = plan.prefix_pieces + plan.own_pieces
+    if plan.own_pieces < 1 or plan.own_pieces > 64 or plan.piece_keys < 1 or not (1 if prefix_len else 0) <= plan.prefix_pieces <= (64 if prefix_len else 0):
+        raise KernelError(f"{who}: the plan does not fit a prefix of {prefix_len} keys")
+    floats = n * n_q_heads * records * head_dim if records > 1 else 0
+    _packed_vector(scratch, "scratch", who, torch.float32, floats + (n * n_q_heads * records * 2 if records > 1 else 0))
+    _on_this_device(who, q=q, k_pages=k_pages, v_pages=v_pages, prefix_pages=prefix_pages, block_tables=block_tables, seq_starts=seq_starts,
+                    positions=positions, out=out, scratch=scratch, status=status)
+    if n == 0 or n_seqs == 0:
+        return
+    part_o = scratch.data_ptr()
+    launch_counts["own"] += (1 if plan.prefix_pieces else 0) + (1 if records > 1 else 0)      # beside the one that every call counts
+    _call(_fn("attention_packed", _elem(q), "erb_attention_shared_prefix"), q, ld_q, k_pages, v_pages, n_pages, page_size, prefix_pages, int(prefix_len),
+          block_tables, block_tables.shape[1], seq_starts, positions, n_seqs, n, out, ld_o, n_q_heads, n_kv_heads, head_dim, float(scale),
+          plan.prefix_pieces, plan.own_pieces, plan.piece_keys, part_o, part_o + 4 * floats, status, _stream())
 
 
 # --- sampling --------------------------------------------------------------------------------

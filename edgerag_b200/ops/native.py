@@ -41,6 +41,8 @@ LIBRARIES: dict[str, tuple[str, tuple[str, ...], bool]] = {
     "attention_tc": ("attention_tc.cu", ("-lcuda",), False),
     "attention_prefill": ("attention_prefill.cu", ("-lcuda",), False),
     "attention_wide": ("attention_wide.cu", ("-lcuda",), False),
+    "rotary": ("rotary.cu", (), True),
+    "attention_packed": ("attention_packed.cu", (), True),
     "gemm": ("gemm.cu", ("-lcublasLt",), True),
     "linear_tc": ("linear_tc.cu", ("-lcuda",), False),
     "sampling": ("sampling.cu", (), False),
