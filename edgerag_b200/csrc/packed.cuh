@@ -93,4 +93,36 @@ __device__ __forceinline__ void key_rows(const PackedArgs& a, const int* table, 
   }
 }
 
+// Joins the records of each (token, head), in their order: a warp each.
+static __global__ void __launch_bounds__(128)
+attention_merge_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml, elem_t* __restrict__ out, long long ld_out,
+                       const int* __restrict__ seq_starts, int n_seqs, int n_tokens, int nq, int D, int n_rec) {
+  chain_wait();
+  const long long item = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  const long long first = seq_starts[0], end = min((long long)seq_starts[n_seqs], (long long)n_tokens);
+  if (first < 0 || item < first * nq || item >= end * nq) return;
+  const float* ml = part_ml + 2 * item * n_rec;
+  float m = -INFINITY;
+  for (int r = lane; r < n_rec; r += 32)
+    if (ml[2 * r + 1] != 0.f) m = fmaxf(m, ml[2 * r]);
+  m = warp_max(m);
+  float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, l = 0.f;
+  for (int r = 0; r < n_rec; ++r) {
+    const float sum = ml[2 * r + 1];
+    if (sum == 0.f) continue;
+    const float w = exp2f(ml[2 * r] - m);
+    l = fmaf(sum, w, l);
+    const float* src = part_o + (item * n_rec + r) * D;
+#pragma unroll
+    for (int c = 0; c < 8; ++c)
+      if (lane + 32 * c < D) o[c] = fmaf(src[lane + 32 * c], w, o[c]);
+  }
+  const float inv = l != 0.f ? 1.f / l : 0.f;
+  elem_t* dst = out + (item / nq) * ld_out + (item % nq) * D;
+#pragma unroll
+  for (int c = 0; c < 8; ++c)
+    if (lane + 32 * c < D) Elem<elem_t>::store(dst + lane + 32 * c, o[c] * inv);
+}
+
 }  // namespace erb

@@ -151,6 +151,11 @@ _SIGNATURES = {
                           c_int, c_int, c_int, c_int, c_void_p, c_void_p],
     "erb_attention_prompt": [c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_int, c_int, c_void_p, c_longlong,
                              c_int, c_int, c_int, c_float, c_void_p, c_void_p],
+    "erb_attention_prompt_tc": [c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_int, c_int, c_void_p, c_longlong,
+                                c_int, c_int, c_int, c_float, c_void_p, c_void_p],
+    "erb_attention_shared_prefix_tc": [c_void_p, c_longlong, c_void_p, c_void_p, c_int, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p,
+                                       c_void_p, c_int, c_int, c_void_p, c_longlong, c_int, c_int, c_int, c_float, c_int, c_int, c_int,
+                                       c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p],
     "erb_attention_shared_prefix": [c_void_p, c_longlong, c_void_p, c_void_p, c_int, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p,
                                     c_void_p, c_int, c_int, c_void_p, c_longlong, c_int, c_int, c_int, c_float, c_int, c_int, c_int,
                                     c_void_p, c_void_p, c_void_p, c_void_p],
@@ -2394,6 +2399,16 @@ def _grouped_heads(who: str, n_q_heads: int, n_kv_heads: int, head_dim: int, sca
         raise KernelError(f"{who}: scale {scale} must be positive")
 
 
+def packed_tc_supported(dtype: torch.dtype, head_dim: int, page_size: int = 16) -> bool:
+    """Shapes that ``attention_prompt`` and ``attention_shared_prefix`` give to the tensor cores (rows and pools on 16-byte boundaries): bfloat16,
+    heads of 64 and 128, pages of 8 to 128 tokens, a power of two.  Everything else goes to the kernels on CUDA cores."""
+    return dtype == torch.bfloat16 and head_dim in (64, 128) and 8 <= page_size <= 128 and page_size & (page_size - 1) == 0
+
+
+def _on_16_bytes(*tensors: torch.Tensor) -> bool:
+    return all(t.data_ptr() % 16 == 0 and (t.dim() != 2 or t.shape[0] <= 1 or t.stride(0) * t.element_size() % 16 == 0) for t in tensors)
+
+
 def attention_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seq_starts: torch.Tensor, out: torch.Tensor, n_q_heads: int,
                      n_kv_heads: int, scale: float, status: torch.Tensor) -> None:
     """Causal attention over whole prompts, packed one behind the other; keys and values lie in rows, not in the cache.
@@ -2418,7 +2433,11 @@ def attention_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seq_star
     _on_this_device(who, q=q, k=k, v=v, seq_starts=seq_starts, out=out, status=status)
     if n == 0 or seq_starts.numel() == 1:
         return
-    _call(_fn("attention_packed", _elem(q), "erb_attention_prompt"), q, ld_q, k, ld_k, v, ld_v, seq_starts, seq_starts.numel() - 1, n, out, ld_o,
+    if packed_tc_supported(q.dtype, head_dim) and _on_16_bytes(q, k, v, out) and min(ld_k, ld_v) >= n_kv_heads * head_dim:
+        fn = _fn("attention_packed_tc", None, "erb_attention_prompt_tc")
+    else:
+        fn = _fn("attention_packed", _elem(q), "erb_attention_prompt")
+    _call(fn, q, ld_q, k, ld_k, v, ld_v, seq_starts, seq_starts.numel() - 1, n, out, ld_o,
           n_q_heads, n_kv_heads, head_dim, float(scale), status, _stream())
 
 
@@ -2429,6 +2448,20 @@ class SharedPrefixPlan(NamedTuple):
     own_pieces: int          # pieces of a request's own keys, of ``piece_keys`` each (the last takes the rest)
     piece_keys: int
     floats: int              # float32 entries of scratch
+    tensor_cores: bool = False
+    prefix_dual: bool = False      # tensor cores: a block's two query tiles are the same 128 rows, each with half of the keys and a piece of
+    own_dual: bool = False         # its own (so a call's blocks cut the keys into half as many pieces)
+
+
+def _cut(tiles: int, blocks: int, sms: int, fixed: int) -> int:
+    """Pieces to cut ``tiles`` tiles of keys into, for ``blocks`` blocks that each walk them, one block a multiprocessor: the number with the
+    shortest run, waves times the tiles of a piece and the ``fixed`` cost of a block (in tiles)."""
+    best, most = None, max(1, min(32, tiles))
+    for pieces in range(1, most + 1):
+        cost = -(-blocks * pieces // sms) * (-(-tiles // pieces) + fixed)
+        if best is None or cost < best[0]:
+            best = (cost, pieces)
+    return best[1]
 
 
 def shared_prefix_plan(n_tokens: int, n_seqs: int, n_q_heads: int, n_kv_heads: int, head_dim: int, dtype: torch.dtype, page_size: int,
@@ -2440,6 +2473,21 @@ def shared_prefix_plan(n_tokens: int, n_seqs: int, n_q_heads: int, n_kv_heads: i
         raise KernelError("shared_prefix_plan: negative sizes")
     sms = _sms(torch.device("cuda", torch._C._cuda_getDevice())) if sms is None else sms
     own_keys = max(1, max_keys - prefix_len)
+    if packed_tc_supported(dtype, head_dim, page_size):
+        group = n_q_heads // n_kv_heads
+        prefix_dual, own_dual = n_tokens * group <= 128, max_tokens * group <= 128
+        prefix_pieces = 0
+        if prefix_len:
+            each = 2 if prefix_dual else 1
+            prefix_pieces = each * _cut(-(-prefix_len // (128 * each)), max(1, n_kv_heads * -(-n_tokens * group // 256)), sms, 3)
+        each = 2 if own_dual else 1
+        tiles = own_keys // 128 + 2 - (prefix_len % 128 == 0)
+        cut = _cut(-(-tiles // each), max(1, n_kv_heads * max(n_seqs, -(-n_tokens * group // 256))), sms, 3)
+        piece_keys = -(-tiles // cut) * 128
+        own_pieces = -(-tiles * 128 // piece_keys) * each
+        records = prefix_pieces + own_pieces
+        return SharedPrefixPlan(prefix_pieces, own_pieces, piece_keys, n_tokens * n_q_heads * records * (head_dim + 2) if records > 1 else 0, True,
+                                prefix_dual, own_dual)
     # Two blocks a multiprocessor, tiles of 64 keys, two tiles a piece at least.
     rows = n_tokens * (n_q_heads // n_kv_heads)
     blocks = max(1, -(-rows // 64) * n_kv_heads)
@@ -2490,7 +2538,7 @@ def attention_shared_prefix(q: torch.Tensor, k_pages: torch.Tensor, v_pages: tor
     if n * (n_q_heads // n_kv_heads) >= 1 << 30 or n_seqs >= 1 << 24:
         raise KernelError(f"{who}: {n} tokens of {n_q_heads} heads in one call")
     records = plan.prefix_pieces + plan.own_pieces
-    if plan.own_pieces < 1 or plan.own_pieces > 64 or plan.piece_keys < 1 or not (1 if prefix_len else 0) <= plan.prefix_pieces <= (64 if prefix_len else 0):
+    if (plan.prefix_dual and plan.prefix_pieces % 2) or (plan.own_dual and plan.own_pieces % 2) or plan.own_pieces < 1 or plan.own_pieces > 64 or plan.piece_keys < 1 or not (1 if prefix_len else 0) <= plan.prefix_pieces <= (64 if prefix_len else 0):
         raise KernelError(f"{who}: the plan does not fit a prefix of {prefix_len} keys")
     floats = n * n_q_heads * records * head_dim if records > 1 else 0
     _packed_vector(scratch, "scratch", who, torch.float32, floats + (n * n_q_heads * records * 2 if records > 1 else 0))
@@ -2500,9 +2548,14 @@ def attention_shared_prefix(q: torch.Tensor, k_pages: torch.Tensor, v_pages: tor
         return
     part_o = scratch.data_ptr()
     launch_counts["own"] += (1 if plan.prefix_pieces else 0) + (1 if records > 1 else 0)      # beside the one that every call counts
-    _call(_fn("attention_packed", _elem(q), "erb_attention_shared_prefix"), q, ld_q, k_pages, v_pages, n_pages, page_size, prefix_pages, int(prefix_len),
-          block_tables, block_tables.shape[1], seq_starts, positions, n_seqs, n, out, ld_o, n_q_heads, n_kv_heads, head_dim, float(scale),
-          plan.prefix_pieces, plan.own_pieces, plan.piece_keys, part_o, part_o + 4 * floats, status, _stream())
+    if plan.tensor_cores and packed_tc_supported(q.dtype, head_dim, page_size) and _on_16_bytes(q, out, k_pages, v_pages, scratch) \
+            and n_pages * n_kv_heads * page_size <= 0x7fffffff:
+        fn, dual, piece_keys = _fn("attention_packed_tc", None, "erb_attention_shared_prefix_tc"), (int(plan.prefix_dual), int(plan.own_dual)), plan.piece_keys
+    else:
+        fn, dual, piece_keys = _fn("attention_packed", _elem(q), "erb_attention_shared_prefix"), (), -(-plan.piece_keys // (2 if plan.own_dual else 1))
+    _call(fn, q, ld_q, k_pages, v_pages, n_pages, page_size, prefix_pages, int(prefix_len), block_tables, block_tables.shape[1], seq_starts, positions, n_seqs,
+          n, out, ld_o, n_q_heads, n_kv_heads, head_dim, float(scale), plan.prefix_pieces, plan.own_pieces, piece_keys, *dual, part_o, part_o + 4 * floats,
+          status, _stream())
 
 
 # --- sampling --------------------------------------------------------------------------------

@@ -43,6 +43,7 @@ LIBRARIES: dict[str, tuple[str, tuple[str, ...], bool]] = {
     "attention_wide": ("attention_wide.cu", ("-lcuda",), False),
     "rotary": ("rotary.cu", (), True),
     "attention_packed": ("attention_packed.cu", (), True),
+    "attention_packed_tc": ("attention_packed_tc.cu", ("-lcuda",), False),
     "gemm": ("gemm.cu", ("-lcublasLt",), True),
     "linear_tc": ("linear_tc.cu", ("-lcuda",), False),
     "sampling": ("sampling.cu", (), False),

@@ -231,6 +231,28 @@ def test_any_cut_gives_the_same(elem, plan):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("plan", [(1, 1, 4096, False, False), (3, 2, 128, False, False), (2, 2, 4096, True, True), (64, 1, 128, True, False),
+                                  (6, 64, 128, True, True), (4, 6, 64, True, True), (2, 3, 256, False, False)])
+def test_any_cut_gives_the_same_on_tensor_cores(dim, plan):
+    c = shared_call("bfloat16", 330, (1, 4, 1, 40), (0, 260, 31, 500), 4, 2, dim, 16)
+    records = plan[0] + plan[1]
+    out, status = run_shared(c, K.SharedPrefixPlan(*plan[:3], 46 * 4 * records * (dim + 2), True, *plan[3:]))
+    assert status == 0
+    check_shared(c, out)
+
+
+@pytest.mark.gpu
+def test_rows_off_16_bytes_take_the_other_kernel():
+    """The plan may be the tensor cores'; rows whose stride they cannot take are computed all the same."""
+    for pad in (8, 3):
+        c = shared_call("bfloat16", 200, (1, 2), (10, 150), 4, 2, 64, 16, pad=pad)
+        out, status = run_shared(c)
+        assert status == 0
+        check_shared(c, out)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("elem,dim", [("bfloat16", 64), ("bfloat16", 128), ("float32", 64), ("bfloat16", 40)])
 def test_places_that_hold_no_keys_stay_unseen(elem, dim):
     """Slots behind a request's last key, behind the prefix in its last page and before the own keys in that page may hold anything."""
