@@ -117,6 +117,142 @@ __global__ void __launch_bounds__(128) rotary_general_kernel(const RotaryArgs a)
       for (int i = lane; i < D; i += 32) Elem<elem_t>::store(to[n] + i, x[i]);
 }
 
+// Sixteen bytes of neighbouring entries as floats, and back.
+template <typename T> struct Piece;
+template <> struct Piece<float> {
+  static constexpr int N = 4;
+  static __device__ __forceinline__ void unpack(const uint4& r, float* v) {
+    v[0] = __uint_as_float(r.x); v[1] = __uint_as_float(r.y); v[2] = __uint_as_float(r.z); v[3] = __uint_as_float(r.w);
+  }
+  static __device__ __forceinline__ uint4 pack(const float* v) {
+    return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+  }
+};
+template <> struct Piece<__nv_bfloat16> {
+  static constexpr int N = 8;
+  static __device__ __forceinline__ void unpack(const uint4& r, float* v) {
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { v[2 * i] = __uint_as_float(w[i] << 16); v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+  }
+  static __device__ __forceinline__ uint4 pack(const float* v) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __nv_bfloat162 two = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&two);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+};
+
+// Rows on 16-byte boundaries, heads of UNITS * 2 N entries (N: sixteen bytes of entries), turned entries a multiple of 2 N.  A unit is two
+// pieces of sixteen bytes that hold whole pairs: neighbours with `pairs`, else piece u of the first half of the turned part and its partner
+// in the second half (behind the turned part: two neighbours).  UNITS neighbouring lanes make a head.  A block works on the units of one
+// token, kAhead for each thread, asked for before the token's angles are made, blockIdx.y telling apart the blocks that share a token.
+constexpr int kFastThreads = 128, kAhead = 2;
+
+template <int UNITS, bool PAIRS>
+__global__ void __launch_bounds__(kFastThreads) rotary_units_kernel(const RotaryArgs a) {
+  using P = Piece<elem_t>;
+  constexpr int N = P::N, D = UNITS * 2 * N;
+  __shared__ float2 trig[D / 2];
+  const int half = a.rot_dim / 2, turned = a.rot_dim / (2 * N);          // units of a head that are turned
+  const int heads = a.nq + (a.k ? a.nkv : 0), q_units = heads * UNITS, all = q_units + (a.v ? a.nkv * UNITS : 0);
+  const int t = blockIdx.x, stride = gridDim.y * kFastThreads;
+  const int u = threadIdx.x % UNITS;                                     // this thread's unit of every head it works on
+  const int o0 = PAIRS ? 2 * u * N : (u < turned ? u * N : a.rot_dim + (u - turned) * 2 * N);
+  const int o1 = PAIRS || u >= turned ? o0 + N : half + u * N;
+  chain_wait();
+  const elem_t* q = a.q + t * a.ld_q;
+  const elem_t* k = a.k + t * a.ld_k;
+  const elem_t* v = a.v + t * a.ld_v;
+  const int position = a.rot_dim ? a.positions[t] : 0;
+  const long long slot = slot_of(a, t, blockIdx.y == 0 && threadIdx.x == 0);
+  const long long cache_row = slot < 0 ? 0 : ((slot / a.page_size) * a.nkv * a.page_size + slot % a.page_size) * D;
+  const long long head_step = (long long)a.page_size * D;                // from a kv head's row of a page to the next head's
+  bool first = true;
+  for (int w0 = blockIdx.y * kFastThreads; w0 < all; w0 += stride * kAhead) {      // (uniform: the lanes of a head stay together)
+    uint4 x0[kAhead], x1[kAhead];
+#pragma unroll
+    for (int n = 0; n < kAhead; ++n) {
+      const int w = w0 + n * stride + threadIdx.x, head = w / UNITS;
+      x0[n] = x1[n] = make_uint4(0, 0, 0, 0);
+      if (w >= all) continue;
+      const elem_t* src = head < a.nq ? q + head * D : (head < heads ? k + (head - a.nq) * D : v + (head - heads) * D);
+      const int p0 = w < q_units ? o0 : 2 * u * N, p1 = w < q_units ? o1 : p0 + N;
+      x0[n] = *reinterpret_cast<const uint4*>(src + p0);
+      x1[n] = *reinterpret_cast<const uint4*>(src + p1);
+    }
+    if (first) {
+      for (int i = threadIdx.x; i < half; i += kFastThreads) turn_of(position, a.turns[i], a.multiplier, trig[i].x, trig[i].y);
+      __syncthreads();
+      first = false;
+    }
+#pragma unroll
+    for (int n = 0; n < kAhead; ++n) {
+      const int w = w0 + n * stride + threadIdx.x, head = w / UNITS;
+      if (w0 + n * stride >= all) break;                                 // (the whole block)
+      float lo[N], hi[N];
+      P::unpack(x0[n], lo);
+      P::unpack(x1[n], hi);
+      const float* weight = w >= q_units ? nullptr : (head < a.nq ? a.q_norm : a.k_norm);
+      if (a.q_norm || a.k_norm) {                                        // (every lane takes part in the exchange)
+        float ss = 0.f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) ss = fmaf(lo[i], lo[i], fmaf(hi[i], hi[i], ss));
+#pragma unroll
+        for (int o = UNITS / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        if (weight) {
+          const float rs = rsqrtf(ss / (float)D + a.eps);
+#pragma unroll
+          for (int i = 0; i < N; ++i) { lo[i] = lo[i] * rs * weight[o0 + i]; hi[i] = hi[i] * rs * weight[o1 + i]; }
+        }
+      }
+      if (w >= all) continue;
+      if (w >= q_units) {                                                // values: to the cache as they are
+        if (slot < 0) continue;
+        elem_t* dst = a.v_pages + cache_row + (head - heads) * head_step + 2 * u * N;
+        *reinterpret_cast<uint4*>(dst) = x0[n];
+        *reinterpret_cast<uint4*>(dst + N) = x1[n];
+        continue;
+      }
+      if (u < turned) {
+        if (PAIRS) {
+#pragma unroll
+          for (int i = 0; i < N; i += 2) {
+            const float2 c0 = trig[u * N + i / 2], c1 = trig[u * N + N / 2 + i / 2];
+            rotate_pair(lo[i], lo[i + 1], c0.x, c0.y, lo[i], lo[i + 1]);
+            rotate_pair(hi[i], hi[i + 1], c1.x, c1.y, hi[i], hi[i + 1]);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < N; ++i) {
+            const float2 c = trig[u * N + i];
+            rotate_pair(lo[i], hi[i], c.x, c.y, lo[i], hi[i]);
+          }
+        }
+      }
+      const uint4 y0 = P::pack(lo), y1 = P::pack(hi);
+      auto store = [&](elem_t* dst) {
+        *reinterpret_cast<uint4*>(dst + o0) = y0;
+        *reinterpret_cast<uint4*>(dst + o1) = y1;
+      };
+      if (head < a.nq) store(a.q_out + t * a.ld_qo + head * D);
+      else {
+        if (a.k_out) store(a.k_out + t * a.ld_ko + (head - a.nq) * D);
+        if (slot >= 0) store(a.k_pages + cache_row + (head - a.nq) * head_step);
+      }
+    }
+  }
+}
+
+template <int UNITS>
+void launch_units(const RotaryArgs& a, dim3 grid, cudaStream_t stream) {
+  if (a.pairs) launch_chained(rotary_units_kernel<UNITS, true>, grid, dim3(kFastThreads), 0, stream, a);
+  else launch_chained(rotary_units_kernel<UNITS, false>, grid, dim3(kFastThreads), 0, stream, a);
+}
+
 }  // namespace
 
 // q, k, v: rows of heads, ld_* elements apart (k null: queries only; v null: no values).  q_out / k_out: rows for the results, the inputs
@@ -136,6 +272,26 @@ ERB_EXPORT int erb_rotary_append(const void* q, void* q_out, long long ld_q, lon
   RotaryArgs a = {(const elem_t*)q, (elem_t*)q_out, ld_q, ld_qo, (const elem_t*)k, (elem_t*)k_out, ld_k, ld_ko, (const elem_t*)v, ld_v,
                   q_norm, k_norm, eps, multiplier, positions, (const unsigned long long*)turns, rot_dim, pairs, slots, (elem_t*)k_pages,
                   (elem_t*)v_pages, (long long)n_pages * page_size, page_size > 0 ? page_size : 1, n_tokens, nq, nkv, head_dim, status};
+  constexpr int N = Piece<elem_t>::N;
+  const int units = head_dim / (2 * N);
+  const uintptr_t all = (uintptr_t)q | (uintptr_t)q_out | (uintptr_t)k | (uintptr_t)k_out | (uintptr_t)v | (uintptr_t)k_pages | (uintptr_t)v_pages;
+  if (head_dim % (2 * N) == 0 && rot_dim % (2 * N) == 0 && units >= 2 && units <= 32 && !(units & (units - 1)) && !(all & 15) &&
+      !((ld_q | ld_qo | ld_k | ld_ko | ld_v) % N)) {
+    const int work = (nq + (k ? nkv : 0) + (v ? nkv : 0)) * units;
+    // As many blocks a token as its units fill, no more than give each multiprocessor sixteen.
+    int share = (work + kFastThreads * kAhead - 1) / (kFastThreads * kAhead);
+    const int want = (sm_count() * 16 + n_tokens - 1) / n_tokens;
+    share = share < want ? share : want;
+    const dim3 grid(n_tokens, share < 1 ? 1 : share);
+    switch (units) {
+      case 2: launch_units<2>(a, grid, (cudaStream_t)stream); break;
+      case 4: launch_units<4>(a, grid, (cudaStream_t)stream); break;
+      case 8: launch_units<8>(a, grid, (cudaStream_t)stream); break;
+      case 16: launch_units<16>(a, grid, (cudaStream_t)stream); break;
+      default: launch_units<32>(a, grid, (cudaStream_t)stream);
+    }
+    return check_launch("rotary_append");
+  }
   const long long items = (long long)n_tokens * (nq + (k ? nkv : 0) + (v ? nkv : 0)), blocks = (items + 3) / 4;
   if (blocks > 0x7fffffffLL) return fail(ERB_ERR_UNSUPPORTED, "rotary_append: %d tokens of %d heads", n_tokens, nq);
   launch_chained(rotary_general_kernel, dim3((unsigned)blocks), dim3(128), 4 * head_dim * sizeof(float), (cudaStream_t)stream, a);
