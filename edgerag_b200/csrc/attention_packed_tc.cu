@@ -31,6 +31,7 @@
 #undef ERB_ELEM
 #define ERB_ELEM 1
 #include "packed.cuh"
+#include "packed_few.cuh"
 #include "tc_common.cuh"
 
 using namespace erb;
@@ -42,6 +43,7 @@ namespace {
 constexpr int BM = 128, BN = 128;
 constexpr int kSoftmaxWarps = 8, kIssueWarp = 8, kCopyWarp = 10, kThreads = 352;
 constexpr float kMoveFrom = 8.f;          // powers of two by which a tile's maximum is above the reference before that moves
+constexpr int kOwnMany = 0, kOwnToken = 1, kOwnRows = 2;      // kernels for a request's own keys
 constexpr int kGaveUp = 9100000;          // status code of a wait that ran out
 
 template <int D> struct Cfg {
@@ -477,6 +479,25 @@ int launch_tc(const PackedArgs& a, const CUtensorMap& mk, const CUtensorMap& mv,
   return a.D == 64 ? launch_one<64, MODE>(a, mk, mv, grid, dual, stream, who) : launch_one<128, MODE>(a, mk, mv, grid, dual, stream, who);
 }
 
+// A request's own keys by the kernels for few rows: rows 1: one token a request (or one after the other), up to 16 query heads a kv head.
+template <int D>
+int launch_few(const PackedArgs& a, bool one_token, int early, cudaStream_t stream, const char* who) {
+  auto kern = one_token ? attention_own_token_kernel<D> : attention_own_rows_kernel<D>;
+  const int bytes = one_token ? (int)FewSmem<D>::kBytes : (int)FewRowsSmem<D>::kBytes;
+  static bool configured[64][2] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return fail(ERB_ERR_CUDA, "%s: no device", who);
+  if (!configured[dev][one_token]) {
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) return fail(ERB_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
+    configured[dev][one_token] = true;
+  }
+  const long long tiles = one_token ? a.n_seqs : (long long)a.n_tokens * (a.nq / a.nkv) / kFewRows + a.n_seqs;
+  if (tiles > 65535 || a.pieces > 65535) return fail(ERB_ERR_UNSUPPORTED, "%s: too many rows", who);
+  launch_chained(kern, dim3(a.nkv, (unsigned)tiles, a.pieces), dim3(kFewThreads), bytes, stream, a, early);
+  return check_launch(who);
+}
+
 bool aligned(const void* p, long long ld) { return ((uintptr_t)p & 15) == 0 && ld % 8 == 0; }
 
 }  // namespace
@@ -504,16 +525,18 @@ ERB_EXPORT int erb_attention_prompt_tc(const void* q, long long ld_q, const void
 }
 
 // The arguments of erb_attention_shared_prefix (attention_packed.cu); heads of 64 or 128, rows, their strides and the pools on 16-byte
-// boundaries, pages of 8 to 128 tokens, a power of two.  prefix_dual / own_dual: blocks own 128 rows and leave two records each, so
-// that prefix_pieces / own_pieces are twice the blocks' pieces.
+// boundaries, pages of 8 to 128 tokens, a power of two.  prefix_dual: blocks own 128 rows and leave two records each, so that prefix_pieces
+// is twice the blocks' pieces.  own: the kernel for a request's own keys (kOwnMany: this file's for many rows; kOwnToken, kOwnRows:
+// packed_few.cuh's, which join the records themselves where own_pieces is 1).
 ERB_EXPORT int erb_attention_shared_prefix_tc(const void* q, long long ld_q, const void* k_pages, const void* v_pages, int n_pages, int page_size,
                                               const int* prefix_pages, int prefix_len, const int* tables, int table_ld, const int* seq_starts,
                                               const int* positions, int n_seqs, int n_tokens, void* out, long long ld_out, int nq, int nkv,
                                               int head_dim, float scale, int prefix_pieces, int own_pieces, int piece_keys, int prefix_dual,
-                                              int own_dual, float* part_o, float* part_ml, int* status, void* stream) {
+                                              int own, float* part_o, float* part_ml, int* status, void* stream) {
   if (n_seqs <= 0 || n_tokens <= 0) return ERB_OK;
   if (nq <= 0 || nkv <= 0 || nq % nkv || !status || n_pages <= 0 || prefix_len < 0 || table_ld <= 0 || prefix_pieces < (prefix_len > 0 ? 1 : 0) ||
-      own_pieces < 1 || piece_keys <= 0 || !(scale > 0.f) || (prefix_dual && prefix_pieces % 2) || (own_dual && own_pieces % 2))
+      own_pieces < 1 || piece_keys <= 0 || !(scale > 0.f) || prefix_pieces > 64 ||
+      (prefix_dual && prefix_pieces % 2) || own < kOwnMany || own > kOwnRows || (own == kOwnToken && nq / nkv > 16))
     return fail(ERB_ERR_ARG, "attention_shared_prefix_tc: bad sizes");
   if ((head_dim != 64 && head_dim != 128) || !aligned(q, ld_q) || !aligned(out, ld_out) || !aligned(k_pages, 0) || !aligned(v_pages, 0) ||
       page_size < 8 || page_size > BN || (page_size & (page_size - 1)) || (unsigned long long)n_pages * nkv * page_size > 0x7fffffffull)
@@ -534,15 +557,19 @@ ERB_EXPORT int erb_attention_shared_prefix_tc(const void* q, long long ld_q, con
   if ((rc = rows_map(&mk, k_pages, pool_rows, head_dim, head_dim, page_size, who)) || (rc = rows_map(&mv, v_pages, pool_rows, head_dim, head_dim, page_size, who)))
     return rc;
   const long long rows = (long long)n_tokens * (nq / nkv);
-  auto tiles = [&](int dual) { return rows / (dual ? BM : 2 * BM); };
   if (prefix_len > 0) {
     a.rec0 = 0;
     a.pieces = prefix_dual ? prefix_pieces / 2 : prefix_pieces;
-    if ((rc = launch_tc<kPrefix>(a, mk, mv, dim3(nkv, (unsigned)min(tiles(prefix_dual) + 1, 1LL << 20), a.pieces), prefix_dual, s, who))) return rc;
+    if ((rc = launch_tc<kPrefix>(a, mk, mv, dim3(nkv, (unsigned)min(rows / (prefix_dual ? BM : 2 * BM) + 1, 1LL << 20), a.pieces), prefix_dual, s, who))) return rc;
   }
   a.rec0 = prefix_len > 0 ? prefix_pieces : 0;
-  a.pieces = own_dual ? own_pieces / 2 : own_pieces;
-  if ((rc = launch_tc<kOwn>(a, mk, mv, dim3(nkv, (unsigned)min(tiles(own_dual) + n_seqs, 1LL << 20), a.pieces), own_dual, s, who)) || n_rec <= 1) return rc;
+  a.pieces = own_pieces;
+  if (own == kOwnMany) {
+    if ((rc = launch_tc<kOwn>(a, mk, mv, dim3(nkv, (unsigned)min(rows / (2 * BM) + n_seqs, 1LL << 20), a.pieces), 0, s, who)) || n_rec <= 1) return rc;
+  } else {
+    rc = head_dim == 64 ? launch_few<64>(a, own == kOwnToken, prefix_len > 0, s, who) : launch_few<128>(a, own == kOwnToken, prefix_len > 0, s, who);
+    if (rc || own_pieces == 1) return rc;
+  }
   const long long blocks = ((long long)n_tokens * nq + 3) / 4;
   if (blocks > 0x7fffffffLL) return fail(ERB_ERR_UNSUPPORTED, "%s: too many rows", who);
   launch_chained(attention_merge_kernel, dim3((unsigned)blocks), dim3(128), 0, s, (const float*)part_o, (const float*)part_ml, (elem_t*)out, ld_out,

@@ -54,7 +54,7 @@ __device__ __forceinline__ void find_tile(const int* __restrict__ seq_starts, in
   tile = 0;
   for (int s0 = 0; s0 < n_seqs; s0 += 32) {
     const int s = s0 + lane;
-    const int len = s < n_seqs ? max(0, seq_starts[s + 1] - seq_starts[s]) : 0;
+    const int len = s < n_seqs ? max(0, __ldcg(seq_starts + s + 1) - __ldcg(seq_starts + s)) : 0;
     const int mine = (int)(((long long)len * G + rows - 1) / rows);
     int upto = mine;
 #pragma unroll

@@ -2449,8 +2449,11 @@ class SharedPrefixPlan(NamedTuple):
     piece_keys: int
     floats: int              # float32 entries of scratch
     tensor_cores: bool = False
-    prefix_dual: bool = False      # tensor cores: a block's two query tiles are the same 128 rows, each with half of the keys and a piece of
-    own_dual: bool = False         # its own (so a call's blocks cut the keys into half as many pieces)
+    prefix_dual: bool = False      # tensor cores: a block's two query tiles are the same 128 rows, each with half of the keys and a record of its own
+    own: int = 0                   # tensor cores: who takes a request's own keys (OWN_MANY, OWN_TOKEN, OWN_ROWS)
+
+
+OWN_MANY, OWN_TOKEN, OWN_ROWS = 0, 1, 2
 
 
 def _cut(tiles: int, blocks: int, sms: int, fixed: int) -> int:
@@ -2474,20 +2477,25 @@ def shared_prefix_plan(n_tokens: int, n_seqs: int, n_q_heads: int, n_kv_heads: i
     sms = _sms(torch.device("cuda", torch._C._cuda_getDevice())) if sms is None else sms
     own_keys = max(1, max_keys - prefix_len)
     if packed_tc_supported(dtype, head_dim, page_size):
-        group = n_q_heads // n_kv_heads
-        prefix_dual, own_dual = n_tokens * group <= 128, max_tokens * group <= 128
-        prefix_pieces = 0
+        group, prefix_pieces = n_q_heads // n_kv_heads, 0
+        prefix_dual = n_tokens * group <= 128
         if prefix_len:
             each = 2 if prefix_dual else 1
             prefix_pieces = each * _cut(-(-prefix_len // (128 * each)), max(1, n_kv_heads * -(-n_tokens * group // 256)), sms, 3)
-        each = 2 if own_dual else 1
-        tiles = own_keys // 128 + 2 - (prefix_len % 128 == 0)
-        cut = _cut(-(-tiles // each), max(1, n_kv_heads * max(n_seqs, -(-n_tokens * group // 256))), sms, 3)
-        piece_keys = -(-tiles // cut) * 128
-        own_pieces = -(-tiles * 128 // piece_keys) * each
+        own = OWN_TOKEN if max_tokens == 1 and group <= 16 else OWN_ROWS if max_tokens * group < 256 else OWN_MANY
+        if own == OWN_MANY:
+            tiles = own_keys // 128 + 2 - (prefix_len % 128 == 0)
+            cut = _cut(tiles, max(1, n_kv_heads * max(n_seqs, -(-n_tokens * group // 256))), sms, 3)
+            piece_keys = -(-tiles // cut) * 128
+        else:       # small blocks, four a multiprocessor; with one piece there is no separate merge
+            blocks = n_kv_heads * max(1, n_seqs if own == OWN_TOKEN else -(-n_tokens * group // 64))
+            cut = min(max(1, 4 * sms // blocks), max(1, own_keys // 512), 64)
+            piece_keys = -(-own_keys // (64 * cut)) * 64
+            tiles = -(-own_keys // 128)
+        own_pieces = max(1, -(-tiles * 128 // piece_keys))
         records = prefix_pieces + own_pieces
         return SharedPrefixPlan(prefix_pieces, own_pieces, piece_keys, n_tokens * n_q_heads * records * (head_dim + 2) if records > 1 else 0, True,
-                                prefix_dual, own_dual)
+                                prefix_dual, own)
     # Two blocks a multiprocessor, tiles of 64 keys, two tiles a piece at least.
     rows = n_tokens * (n_q_heads // n_kv_heads)
     blocks = max(1, -(-rows // 64) * n_kv_heads)
@@ -2538,7 +2546,7 @@ def attention_shared_prefix(q: torch.Tensor, k_pages: torch.Tensor, v_pages: tor
     if n * (n_q_heads // n_kv_heads) >= 1 << 30 or n_seqs >= 1 << 24:
         raise KernelError(f"{who}: {n} tokens of {n_q_heads} heads in one call")
     records = plan.prefix_pieces + plan.own_pieces
-    if (plan.prefix_dual and plan.prefix_pieces % 2) or (plan.own_dual and plan.own_pieces % 2) or plan.own_pieces < 1 or plan.own_pieces > 64 or plan.piece_keys < 1 or not (1 if prefix_len else 0) <= plan.prefix_pieces <= (64 if prefix_len else 0):
+    if (plan.prefix_dual and plan.prefix_pieces % 2) or (plan.own == OWN_TOKEN and n_q_heads // n_kv_heads > 16) or plan.own not in (OWN_MANY, OWN_TOKEN, OWN_ROWS) or plan.own_pieces < 1 or plan.own_pieces > 64 or plan.piece_keys < 1 or not (1 if prefix_len else 0) <= plan.prefix_pieces <= (64 if prefix_len else 0):
         raise KernelError(f"{who}: the plan does not fit a prefix of {prefix_len} keys")
     floats = n * n_q_heads * records * head_dim if records > 1 else 0
     _packed_vector(scratch, "scratch", who, torch.float32, floats + (n * n_q_heads * records * 2 if records > 1 else 0))
@@ -2547,15 +2555,16 @@ def attention_shared_prefix(q: torch.Tensor, k_pages: torch.Tensor, v_pages: tor
     if n == 0 or n_seqs == 0:
         return
     part_o = scratch.data_ptr()
-    launch_counts["own"] += (1 if plan.prefix_pieces else 0) + (1 if records > 1 else 0)      # beside the one that every call counts
     if plan.tensor_cores and packed_tc_supported(q.dtype, head_dim, page_size) and _on_16_bytes(q, out, k_pages, v_pages, scratch) \
             and n_pages * n_kv_heads * page_size <= 0x7fffffff:
-        fn, dual, piece_keys = _fn("attention_packed_tc", None, "erb_attention_shared_prefix_tc"), (int(plan.prefix_dual), int(plan.own_dual)), plan.piece_keys
+        fn, how = _fn("attention_packed_tc", None, "erb_attention_shared_prefix_tc"), (int(plan.prefix_dual), plan.own)
     else:
-        fn, dual, piece_keys = _fn("attention_packed", _elem(q), "erb_attention_shared_prefix"), (), -(-plan.piece_keys // (2 if plan.own_dual else 1))
+        fn, how = _fn("attention_packed", _elem(q), "erb_attention_shared_prefix"), ()
     _call(fn, q, ld_q, k_pages, v_pages, n_pages, page_size, prefix_pages, int(prefix_len), block_tables, block_tables.shape[1], seq_starts, positions, n_seqs,
-          n, out, ld_o, n_q_heads, n_kv_heads, head_dim, float(scale), plan.prefix_pieces, plan.own_pieces, piece_keys, *dual, part_o, part_o + 4 * floats,
+          n, out, ld_o, n_q_heads, n_kv_heads, head_dim, float(scale), plan.prefix_pieces, plan.own_pieces, plan.piece_keys, *how, part_o, part_o + 4 * floats,
           status, _stream())
+    joined = how and plan.own != OWN_MANY and plan.own_pieces == 1         # by the kernel for the own keys
+    launch_counts["own"] += (1 if plan.prefix_pieces else 0) + (1 if records > 1 and not joined else 0)      # beside the one that every call counts
 
 
 # --- sampling --------------------------------------------------------------------------------
