@@ -2399,10 +2399,10 @@ def _grouped_heads(who: str, n_q_heads: int, n_kv_heads: int, head_dim: int, sca
         raise KernelError(f"{who}: scale {scale} must be positive")
 
 
-def packed_tc_supported(dtype: torch.dtype, head_dim: int, page_size: int = 16) -> bool:
+def packed_tc_supported(dtype: torch.dtype, head_dim: int, group: int, page_size: int = 16) -> bool:
     """Shapes that ``attention_prompt`` and ``attention_shared_prefix`` give to the tensor cores (rows and pools on 16-byte boundaries): bfloat16,
-    heads of 64 and 128, pages of 8 to 128 tokens, a power of two.  Everything else goes to the kernels on CUDA cores."""
-    return dtype == torch.bfloat16 and head_dim in (64, 128) and 8 <= page_size <= 128 and page_size & (page_size - 1) == 0
+    heads of 64 and 128, at most 128 query heads a kv head (``group``), pages of 8 to 128 tokens, a power of two.  Everything else goes to the kernels on CUDA cores."""
+    return dtype == torch.bfloat16 and head_dim in (64, 128) and group <= 128 and 8 <= page_size <= 128 and page_size & (page_size - 1) == 0
 
 
 def _on_16_bytes(*tensors: torch.Tensor) -> bool:
@@ -2433,7 +2433,7 @@ def attention_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seq_star
     _on_this_device(who, q=q, k=k, v=v, seq_starts=seq_starts, out=out, status=status)
     if n == 0 or seq_starts.numel() == 1:
         return
-    if packed_tc_supported(q.dtype, head_dim) and _on_16_bytes(q, k, v, out) and min(ld_k, ld_v) >= n_kv_heads * head_dim:
+    if packed_tc_supported(q.dtype, head_dim, n_q_heads // n_kv_heads) and _on_16_bytes(q, k, v, out) and min(ld_k, ld_v) >= n_kv_heads * head_dim:
         fn = _fn("attention_packed_tc", None, "erb_attention_prompt_tc")
     else:
         fn = _fn("attention_packed", _elem(q), "erb_attention_prompt")
@@ -2476,16 +2476,17 @@ def shared_prefix_plan(n_tokens: int, n_seqs: int, n_q_heads: int, n_kv_heads: i
         raise KernelError("shared_prefix_plan: negative sizes")
     sms = _sms(torch.device("cuda", torch._C._cuda_getDevice())) if sms is None else sms
     own_keys = max(1, max_keys - prefix_len)
-    if packed_tc_supported(dtype, head_dim, page_size):
+    if packed_tc_supported(dtype, head_dim, n_q_heads // n_kv_heads, page_size):
         group, prefix_pieces = n_q_heads // n_kv_heads, 0
-        prefix_dual = n_tokens * group <= 128
+        tile = 128 // group * group            # rows of a query tile: whole tokens
+        prefix_dual = n_tokens * group <= tile
         if prefix_len:
             each = 2 if prefix_dual else 1
-            prefix_pieces = each * _cut(-(-prefix_len // (128 * each)), max(1, n_kv_heads * -(-n_tokens * group // 256)), sms, 3)
+            prefix_pieces = each * _cut(-(-prefix_len // (128 * each)), max(1, n_kv_heads * -(-n_tokens * group // (2 * tile))), sms, 3)
         own = OWN_TOKEN if max_tokens == 1 and group <= 16 else OWN_ROWS if max_tokens * group < 256 else OWN_MANY
         if own == OWN_MANY:
             tiles = own_keys // 128 + 2 - (prefix_len % 128 == 0)
-            cut = _cut(tiles, max(1, n_kv_heads * max(n_seqs, -(-n_tokens * group // 256))), sms, 3)
+            cut = _cut(tiles, max(1, n_kv_heads * max(n_seqs, -(-n_tokens * group // (2 * tile)))), sms, 3)
             piece_keys = -(-tiles // cut) * 128
         else:       # small blocks, four a multiprocessor; with one piece there is no separate merge
             blocks = n_kv_heads * max(1, n_seqs if own == OWN_TOKEN else -(-n_tokens * group // 64))
@@ -2555,7 +2556,7 @@ def attention_shared_prefix(q: torch.Tensor, k_pages: torch.Tensor, v_pages: tor
     if n == 0 or n_seqs == 0:
         return
     part_o = scratch.data_ptr()
-    if plan.tensor_cores and packed_tc_supported(q.dtype, head_dim, page_size) and _on_16_bytes(q, out, k_pages, v_pages, scratch) \
+    if plan.tensor_cores and packed_tc_supported(q.dtype, head_dim, n_q_heads // n_kv_heads, page_size) and _on_16_bytes(q, out, k_pages, v_pages, scratch) \
             and n_pages * n_kv_heads * page_size <= 0x7fffffff:
         fn, how = _fn("attention_packed_tc", None, "erb_attention_shared_prefix_tc"), (int(plan.prefix_dual), plan.own)
     else:
