@@ -10,14 +10,14 @@
 // alike).  Its warps work by role, each as far ahead as the barriers let it, so that a piece's first copies and products run while the
 // one before is being finished:
 //
-//   warp 9 (copy)       finds the pieces and describes them to the others; brings Q tiles, and K and V tiles in turn into one ring of
+//   warp 10 (copy)      finds the pieces and describes them to the others; brings Q tiles, and K and V tiles in turn into one ring of
 //                       shared memory, by TMA tensor copies (128-byte swizzle): from the pages, one copy per page and 64 columns, or from
 //                       rows beside the queries
-//   warp 8 (issue)      S_t = Q_t K^T (M 128, N 128) and O_t += P_t V (M 128, N D, P from TMEM), A and B in turn: while the softmax of
-//                       one runs the tensor cores work for the other
+//   warps 8, 9 (issue)  S_t = Q_t K^T (M 128, N 128) and O_t += P_t V (M 128, N D, P from TMEM), a warp for each query tile: a product
+//                       starts some 300 clocks after what it waits for, which one warp for both would leave the tensor cores idle
 //   warps 0-3, 4-7      softmax of tile A and of tile B: a thread owns a row, takes its 128 scores into registers, and writes P back
 //                       rounded to bfloat16 (the second product's operand type; the sum of P is taken before that rounding, in float)
-//   warps 10, 11        look over the values of tiles with hidden keys (below)
+//   warp 11 (look)      looks over the values of tiles with hidden keys (below)
 //
 // A row's reference maximum moves only when a tile's maximum is 2^8 above it; O is rescaled in TMEM then.  P is a floating-point number, so
 // a reference that is low by eight powers of two costs no precision.
@@ -48,7 +48,7 @@ ERB_DEFINE_LAST_ERROR(erb_last_error)
 namespace {
 
 constexpr int BM = 128, BN = 128;
-constexpr int kSoftmaxWarps = 8, kIssueWarp = 8, kCopyWarp = 9, kLookWarp = 10, kThreads = 384;
+constexpr int kSoftmaxWarps = 8, kIssueWarp = 8, kCopyWarp = 10, kLookWarp = 11, kThreads = 384;
 constexpr int kSoftmaxRegs = 208, kOtherRegs = 88;
 constexpr float kMoveFrom = 8.f;          // powers of two by which a tile's maximum is above the reference before that moves
 constexpr int kOwnMany = 0, kOwnToken = 1, kOwnRows = 2;      // kernels for a request's own keys
@@ -58,17 +58,18 @@ constexpr int kPieces = 4;                // descriptions of pieces of work on t
 template <int D> struct Cfg {
   static constexpr int kHalves = D / 64;                         // blocks of 64 columns (128 bytes of a row)
   static constexpr uint32_t kBlock = BM * 128, kTile = kHalves * kBlock;
-  static constexpr int kStages = D == 64 ? 10 : 4;               // tiles of K or V in the ring
+  static constexpr int kStages = D == 64 ? 8 : 4;                // tiles of K or V in the ring (a power of two)
+  static constexpr int kSets = D == 64 ? 2 : 1;                  // pairs of Q tiles
   static constexpr bool kPlaceForP = D == 64;
   static constexpr uint32_t kColP = 256, kColO = D == 64 ? 384 : 256;
   static constexpr uint32_t kOutBytes = 2048;                    // a softmax warp's place for results on their way out: 32 rows of 64 bytes
   static_assert(kStages % 2 == 0, "a place of the ring holds keys or values, never both");
   // barriers: ring full and empty; descriptions full and empty; a ring place's values looked over; per query tile: queries there and used, scores there,
-  // scores in registers, P written, P V done
+  // scores in registers, each half of P written, P V done
   static constexpr int kFull = 0, kEmpty = kStages, kTold = 2 * kStages, kTaken = kTold + kPieces, kClean = kTaken + kPieces, kQ = kClean + kStages,
-                       kQUsed = kQ + 2, kS = kQ + 4, kRead = kQ + 6, kP = kQ + 8, kPv = kQ + 10, kNumBars = kQ + 12;
-  static constexpr uint32_t kSmemTiles = (2 + kStages) * kTile, kSmemOut = kSmemTiles + kSoftmaxWarps * kOutBytes;
-  static constexpr uint32_t kSmemBytes = kSmemOut + 8 * kNumBars + 16 + kPieces * 64 + 1024;
+                       kQUsed = kQ + 2 * kSets, kS = kQUsed + 2 * kSets, kRead = kS + 2, kP = kS + 4, kPv = kS + 8, kNumBars = kS + 10;
+  static constexpr uint32_t kRing = 2 * kSets * kTile, kSmemTiles = kRing + kStages * kTile, kSmemOut = kSmemTiles + kSoftmaxWarps * kOutBytes;
+  static constexpr uint32_t kSmemBytes = kSmemOut + 8 * kNumBars + 16 + kPieces * 64 + 32 + 1024;
 };
 
 // A piece of work: rows r0 .. r0 + rows of the (token, head) pairs of the tokens from t0 on, key tiles j0 .. j0 + copied.
@@ -82,16 +83,36 @@ struct Piece {
 };
 static_assert(sizeof(Piece) <= 64, "a description's place");
 
-__device__ __forceinline__ bool any_not_finite(const uint4& w) {
-  // a half of a word whose exponent is all ones leaves a zero in x; (x - 1) & ~x has its top bit set where a half is zero
-  const uint32_t e[4] = {w.x, w.y, w.z, w.w};
-  uint32_t hit = 0;
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const uint32_t x = (e[k] & 0x7f807f80u) ^ 0x7f807f80u;
-    hit |= (x - 0x00010001u) & ~x;
+// acc + 0 * w for eight values: stays zero unless one of them is no number.
+__device__ __forceinline__ void gather_not_finite(__nv_bfloat162& acc, const uint4& w) {
+  const __nv_bfloat162 zero = __floats2bfloat162_rn(0.f, 0.f);
+  acc = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&w.x), zero, acc);
+  acc = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&w.y), zero, acc);
+  acc = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&w.z), zero, acc);
+  acc = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&w.w), zero, acc);
+}
+
+// Some tries of a phase, without a look at anything else: a wait that finds its phase complete costs a try and a vote.
+__device__ __forceinline__ bool mbar_try_some(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .u32 n;\n\tmov.u32 n, 0;\n"
+      "TRY_AGAIN:\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t@p bra TRY_DONE;\n\t"
+      "add.u32 n, n, 1;\n\tsetp.lt.u32 p, n, 64;\n\t@p bra TRY_AGAIN;\n\tsetp.ne.u32 p, n, n;\n"
+      "TRY_DONE:\n\tselp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(done)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return done != 0;
+}
+// The rest of a wait: until the phase is there, another warp has given up, or the limit is reached.  The same answer for every lane.
+__device__ __forceinline__ bool wait_long(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+  for (uint32_t i = 0; i < kSpinLimit / 64; ++i) {
+    if (__all_sync(0xffffffffu, mbar_try_some(bar, parity))) return true;
+    if (__any_sync(0xffffffffu, *abort_flag != 0)) return false;
   }
-  return (hit & 0x80008000u) != 0;
+  *abort_flag = 1;
+  return false;
 }
 
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
@@ -105,7 +126,7 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
 struct TileList {
   const int* starts;
   int n_seqs, G, rows, total, most;
-  int first_of_lane;              // tiles of sequence `lane`
+  int first_of_lane, start_of_lane, len_of_lane;              // of sequence `lane`
   __device__ __forceinline__ int tiles(int s) const {
     if (s >= n_seqs) return 0;
     const long long pairs = (long long)max(0, __ldcg(starts + s + 1) - __ldcg(starts + s)) * G;
@@ -113,7 +134,9 @@ struct TileList {
   }
   __device__ __forceinline__ int of(int s0) const { return s0 == 0 ? first_of_lane : tiles(s0 + (int)(threadIdx.x & 31)); }
   __device__ __forceinline__ TileList(const int* starts, int n_seqs, int G, int rows) : starts(starts), n_seqs(n_seqs), G(G), rows(rows) {
-    first_of_lane = tiles(threadIdx.x & 31);
+    start_of_lane = n_seqs > 0 ? __ldcg(starts + min((int)(threadIdx.x & 31), n_seqs - 1)) : 0;
+    len_of_lane = (int)(threadIdx.x & 31) < n_seqs ? __ldcg(starts + (threadIdx.x & 31) + 1) - start_of_lane : 0;
+    first_of_lane = (int)(((long long)max(0, len_of_lane) * G + rows - 1) / rows);
     long long sum = 0;
     most = 0;
     for (int s0 = 0; s0 < n_seqs; s0 += 32) {
@@ -142,7 +165,8 @@ struct TileList {
       const unsigned have = __ballot_sync(0xffffffffu, of(s0) > low);
       const int count = __popc(have);
       if (index < count) {
-        seq = s0 + __fns(have, 0, index + 1);
+        const int lane = threadIdx.x & 31;
+        seq = s0 + __ffs(__ballot_sync(0xffffffffu, (have >> lane & 1) && __popc(have & ((1u << lane) - 1)) == index)) - 1;
         return;
       }
       index -= count;
@@ -159,26 +183,28 @@ attention_packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
   uint8_t* smem = smem_raw + (base - raw);
-  const uint32_t sQ = base, sRing = base + 2 * C::kTile, bars = base + C::kSmemOut;
+  const uint32_t sQ = base, sRing = base + C::kRing, bars = base + C::kSmemOut;
   volatile int* s_abort = reinterpret_cast<volatile int*>(smem + C::kSmemOut + 8 * C::kNumBars);
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(smem + C::kSmemOut + 8 * C::kNumBars + 8);
   auto bar = [&](int which) { return bars + 8u * (uint32_t)which; };
   auto piece_at = [&](int k) { return reinterpret_cast<Piece*>(smem + C::kSmemOut + 8 * C::kNumBars + 16 + (k % kPieces) * 64); };
+  volatile int* s_turn = reinterpret_cast<volatile int*>(smem + C::kSmemOut + 8 * C::kNumBars + 16 + kPieces * 64);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int G = a.nq / a.nkv, RT = BM / G * G, per_piece = dual ? RT : 2 * RT;      // rows of a query tile (whole tokens), of a piece
 
   if (tid == 0) {
-    for (int s = 0; s < C::kStages; ++s) { mbar_init(bar(C::kFull + s), 1); mbar_init(bar(C::kEmpty + s), 1); mbar_init(bar(C::kClean + s), 2); }
+    for (int s = 0; s < C::kStages; ++s) { mbar_init(bar(C::kFull + s), 1); mbar_init(bar(C::kEmpty + s), dual ? 1 : 2); mbar_init(bar(C::kClean + s), 1); }
     for (int k = 0; k < kPieces; ++k) { mbar_init(bar(C::kTold + k), 1); mbar_init(bar(C::kTaken + k), kSoftmaxWarps + 3); }
     for (int t = 0; t < 2; ++t) {
-      mbar_init(bar(C::kQ + t), 1);
-      mbar_init(bar(C::kQUsed + t), 1);
+      for (int s = 0; s < C::kSets; ++s) { mbar_init(bar(C::kQ + 2 * s + t), 1); mbar_init(bar(C::kQUsed + 2 * s + t), dual ? 2 : 1); }
       mbar_init(bar(C::kS + t), 1);
       mbar_init(bar(C::kRead + t), 4);
       mbar_init(bar(C::kP + t), 4);
+      mbar_init(bar(C::kP + 2 + t), 4);
       mbar_init(bar(C::kPv + t), 1);
     }
     *s_abort = 0;
+    for (int w = 0; w < kSoftmaxWarps; ++w) s_turn[w] = 0;
     mbar_init_fence();
   }
   if (warp == kIssueWarp) {
@@ -193,8 +219,7 @@ attention_packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
 
   bool ok = true;                        // the same for a whole warp
   auto wait = [&](int which, int phase) {
-    if (ok) ok = mbar_wait_or_abort(bar(which), phase & 1, s_abort);
-    ok = __all_sync(0xffffffffu, ok) != 0;
+    if (ok && !__all_sync(0xffffffffu, mbar_try_some(bar(which), phase & 1))) ok = wait_long(bar(which), phase & 1, s_abort);
     return ok;
   };
   auto copy_of = [&](int t, int i) { return dual ? 2 * i + t : i; };
@@ -232,43 +257,48 @@ attention_packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
     }
     const TileList list(a.seq_starts, MODE == kPrefix ? 0 : a.n_seqs, G, per_piece);
     if (MODE != kPrefix) total = list.total;
-    total *= (long long)a.nkv * a.pieces;
+    total = min(total * a.nkv * a.pieces, 0x7fffffffLL - (long long)gridDim.x);        // (the launch refuses more)
     int n_told = 0;
     for (int round = 0; ok; ++round) {
-      const long long base_index = (long long)round * gridDim.x;
-      const long long index = base_index + ((round & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+      const int base_index = round * (int)gridDim.x, index = base_index + (int)((round & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
       Piece p = {};
       p.more = base_index < total;
       if (p.more) {
         if (index >= total) continue;
-        p.kvh = (int)(index % a.nkv);
-        p.part = (int)(index / a.nkv % a.pieces);
-        int tile = (int)(index / a.nkv / a.pieces), len;
+        const int rest = index / a.nkv;
+        p.kvh = index - rest * a.nkv;
+        int tile = rest / a.pieces, len;
+        p.part = rest - tile * a.pieces;
         if (MODE == kPrefix) {
           p.t0 = first;
           len = end - first;
         } else {
           list.find(tile, p.seq, tile);
           if (p.seq < 0) continue;
-          p.t0 = __ldcg(a.seq_starts + p.seq);
-          len = __ldcg(a.seq_starts + p.seq + 1) - p.t0;
+          if (p.seq < 32) {
+            p.t0 = __shfl_sync(0xffffffffu, list.start_of_lane, p.seq);
+            len = __shfl_sync(0xffffffffu, list.len_of_lane, p.seq);
+          } else {
+            p.t0 = __ldcg(a.seq_starts + p.seq);
+            len = __ldcg(a.seq_starts + p.seq + 1) - p.t0;
+          }
           if (p.t0 < 0 || p.t0 + (long long)len > a.n_tokens) {
             if (lane == 0) report(a.status, kBadStarts);
             continue;
           }
         }
-        const long long r0 = (long long)tile * per_piece;
-        p.rows = (int)min((long long)per_piece, (long long)len * G - r0);
-        p.token0 = p.t0 + (int)(r0 / G);
+        const int r0 = tile * per_piece, token_tile = RT / G;                  // (tokens times G is below 2^30)
+        p.rows = min(per_piece, len * G - r0);
+        p.token0 = p.t0 + tile * (dual ? token_tile : 2 * token_tile);
         // the keys that the rows of each query tile see
         int most[2] = {0, 0};
         p.least[0] = p.least[1] = INT_MAX;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          const int skip = dual ? 0 : t * RT, n_tokens = max(0, min(RT, p.rows - skip)) / G;     // (rows are whole tokens)
+          const int before = dual ? 0 : t * token_tile, n_tokens = max(0, min(token_tile, min((dual ? 1 : 2) * token_tile, p.t0 + len - p.token0) - before));
           if (MODE == kPrompt) {
             if (n_tokens > 0) {
-              p.least[t] = p.token0 - p.t0 + skip / G + 1;
+              p.least[t] = p.token0 - p.t0 + before + 1;
               most[t] = p.least[t] + n_tokens - 1;
             }
           }
@@ -276,7 +306,7 @@ attention_packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
             int lim = 0;
             const bool mine = i0 + lane < n_tokens;
             if (mine) {
-              lim = max(0, min(__ldcg(a.positions + p.token0 + skip / G + i0 + lane), INT_MAX - 1) + 1);
+              lim = max(0, min(__ldcg(a.positions + p.token0 + before + i0 + lane), INT_MAX - 1) + 1);
               if (MODE == kPrefix) lim = min(lim, a.prefix_len);
               else if (lim > (long long)a.table_ld * a.page_size) { report(a.status, kBadPage); lim = a.table_ld * a.page_size; }
             }
@@ -308,13 +338,13 @@ attention_packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
       if (!p.more) break;
       // queries: whole tokens, the heads of the group in order (tokens behind the sequence's last one are rows that nobody stores)
       for (int t = 0; t < (dual ? 1 : 2); ++t) {
-        if (p.n[t] == 0 && !(dual && p.n[1])) continue;
-        if (copies_q[t] > 0 && !wait(C::kQUsed + t, copies_q[t] - 1)) break;
-        if (lane == 0) {
-          mbar_expect(bar(C::kQ + t), C::kHalves * RT * 128);
-          for (int h = 0; h < C::kHalves; ++h)
-            tma_load_3d(sQ + t * C::kTile + h * C::kBlock, &map_q, 64 * h, p.kvh * G, p.token0 + t * (RT / G), bar(C::kQ + t));
-        }
+        if (p.n[t] == 0) continue;
+        const int set = copies_q[t] % C::kSets, use = copies_q[t] / C::kSets;
+        if (use > 0 && !wait(C::kQUsed + 2 * set + t, use - 1)) break;
+        if (lane == 0) mbar_expect(bar(C::kQ + 2 * set + t), C::kHalves * RT * 128);
+        __syncwarp();
+        if (lane < C::kHalves)
+          tma_load_3d(sQ + (2 * set + t) * C::kTile + lane * C::kBlock, &map_q, 64 * lane, p.kvh * G, p.token0 + t * (RT / G), bar(C::kQ + 2 * set + t));
         ++copies_q[t];
       }
       auto wait_empty = [&](int n) { return n < C::kStages ? ok : wait(C::kEmpty + n % C::kStages, n / C::kStages - 1); };
@@ -356,71 +386,76 @@ attention_packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
         }
       }
     }
-  } else if (warp == kIssueWarp) {
-    // ---- all products; an elected lane issues ----
+  } else if (warp < kCopyWarp) {
+    // ---- the products of a query tile; an elected lane issues, with what a product takes in uniform registers (a shuffle from lane 0 makes them so: a
+    // lane that moves its own values there takes sixty clocks a product) ----
     const bool elected = elect_one();
-    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+    auto uniform = [](uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); };
+    const uint32_t tm = uniform(tmem);
     constexpr uint32_t kIdescS = mma_idesc(BM, BN, false), kIdescO = mma_idesc(BM, D, true);
-    const uint64_t dq0 = make_desc(sQ), dk0 = make_desc(sRing);
-    const uint64_t dv0 = (dk0 & ~((uint64_t)0x3fff << 16)) | ((uint64_t)(C::kBlock >> 4) << 16);      // 64 columns of V apart: a block
-    int ring = 0, steps[2] = {0, 0}, queries[2] = {0, 0};      // ring tiles, steps, Q tiles of the pieces before
+    const uint64_t like = make_desc(0);                        // a descriptor without its address, which is the low 14 bits
+    const uint32_t dq0 = uniform(sQ >> 4), dk0 = uniform(sRing >> 4);
+    auto desc = [&](uint32_t address) { return like | (uint64_t)address; };
+    auto desc_v = [&](uint32_t address) {                      // 64 columns of V apart: a block
+      return (like & ~((uint64_t)0x3fff << 16)) | ((uint64_t)(C::kBlock >> 4) << 16) | (uint64_t)address;
+    };
+    const int t = uniform(warp - kIssueWarp), q_tile = dual ? 0 : t;
+    const uint32_t d_s = tm + t * BN, a_p = C::kPlaceForP ? tm + C::kColP + t * 64 : d_s, d_o = tm + C::kColO + t * D;
+    int ring = 0, steps = 0, queries = 0;                      // ring tiles, steps, Q tiles of the pieces before
     for (int k = 0; wait(C::kTold + k % kPieces, k / kPieces); ++k) {
       const Piece& p = *piece_at(k);
       if (!p.more) break;
-      const int n0 = __shfl_sync(0xffffffffu, p.n[0], 0), n1 = __shfl_sync(0xffffffffu, p.n[1], 0), copied = __shfl_sync(0xffffffffu, p.copied, 0);
-      auto n_of = [&](int t) { return t ? n1 : n0; };
-      // step i of query tile t; `last`: no other product uses these keys afterwards
-      auto scores = [&](int t, int i) {
-        const int g = steps[t] + i, slot = ring + 2 * copy_of(t, i), st = slot % C::kStages;
-        if (g > 0 && !wait((C::kPlaceForP ? C::kRead : C::kPv) + t, g - 1)) return;       // the scores' place is free
+      const int n = uniform(p.n[t]), copied = uniform(p.copied), set = queries % C::kSets;
+      const uint32_t dq = dq0 + uniform(2 * set + q_tile) * (C::kTile >> 4);
+      auto scores = [&](int i) {
+        const int slot = ring + 2 * copy_of(t, i), st = uniform(slot % C::kStages);
         if (!wait(C::kFull + st, slot / C::kStages)) return;
+        if (steps + i > 0 && !wait((C::kPlaceForP ? C::kRead : C::kPv) + t, steps + i - 1)) return;       // the scores' place is free
         fence_after_sync();
+        const uint32_t dk = dk0 + st * (C::kTile >> 4);
         if (elected) {
-          const uint64_t dk = dk0 + (uint64_t)(st * (C::kTile >> 4)), dq = dq0 + (uint64_t)((dual ? 0 : t) * (C::kTile >> 4));
-          const uint32_t d_s = tm + t * BN;
 #pragma unroll
           for (int k = 0; k < D / 16; ++k) {
-            const uint64_t step = (k >> 2) * (C::kBlock >> 4) + 2 * (k & 3);
-            mma_bf16(d_s, dq + step, dk + step, kIdescS, k > 0);
+            const uint32_t step = (k >> 2) * (C::kBlock >> 4) + 2 * (k & 3);
+            mma_bf16(d_s, desc(dq + step), desc(dk + step), kIdescS, k > 0);
           }
-          if (dual || t == 1 || i >= n1) mma_commit(bar(C::kEmpty + st));
           mma_commit(bar(C::kS + t));
-          if (dual ? 2 * i + t + 1 == copied : i + 1 == n_of(t)) mma_commit(bar(C::kQUsed + (dual ? 0 : t)));
+          mma_commit(bar(C::kEmpty + st));
+          if (i + 1 == n) mma_commit(bar(C::kQUsed + 2 * set + q_tile));
         }
         __syncwarp();
       };
-      auto result = [&](int t, int i) {
-        const int g = steps[t] + i, slot = ring + 2 * copy_of(t, i) + 1, st = slot % C::kStages;
-        if (!wait(C::kP + t, g) || !wait(C::kClean + st, slot / C::kStages)) return;
-        fence_after_sync();
-        if (elected) {
-          const uint64_t dv = dv0 + (uint64_t)(st * (C::kTile >> 4));
-          const uint32_t a_p = C::kPlaceForP ? tm + C::kColP + t * 64 : tm + t * BN, d_o = tm + C::kColO + t * D;
-#pragma unroll
-          for (int k = 0; k < BN / 16; ++k) mma_bf16_a_tmem(d_o, a_p + k * 8, dv + (uint64_t)(k * (2048 >> 4)), kIdescO, (k > 0 || i > 0) ? 1u : 0u);
-          if (dual || t == 1 || i >= n1) mma_commit(bar(C::kEmpty + st));
-          mma_commit(bar(C::kPv + t));
-        }
-        __syncwarp();
-      };
-      for (int t = 0; t < 2 && ok; ++t)
-        if (n_of(t) > 0) {
-          if (!(dual && t == 1)) {
-            if (!wait(C::kQ + t, queries[t])) break;
-            ++queries[t];
-          }
-          scores(t, 0);
-        }
-      for (int i = 0; i < max(n0, n1) && ok; ++i) {
-        for (int t = 0; t < 2; ++t) {
-          if (i >= n_of(t)) continue;
-          if (C::kPlaceForP && i + 1 < n_of(t)) scores(t, i + 1);
-          if (ok) result(t, i);
-          if (!C::kPlaceForP && ok && i + 1 < n_of(t)) scores(t, i + 1);
-        }
+      if (p.n[q_tile] > 0) {
+        wait(C::kQ + 2 * set + q_tile, queries / C::kSets);
+        ++queries;
+        if (n == 0 && lane == 0) mbar_arrive(bar(C::kQUsed + 2 * set + q_tile));
       }
-      steps[0] += n0;
-      steps[1] += n1;
+      if (ok && n > 0) scores(0);
+      for (int i = 0; i < n && ok; ++i) {
+        if (C::kPlaceForP && i + 1 < n) scores(i + 1);
+        const int slot = ring + 2 * copy_of(t, i) + 1, st = uniform(slot % C::kStages);
+        if (!wait(C::kClean + st, slot / C::kStages) || !wait(C::kP + t, steps + i)) break;
+        const uint32_t dv = dk0 + st * (C::kTile >> 4), more = uniform(i > 0);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {                           // (the first half of the keys while the second half's weights are made)
+          if (h && !wait(C::kP + 2 + t, steps + i)) break;
+          fence_after_sync();
+          if (elected) {
+#pragma unroll
+            for (int k = 4 * h; k < 4 * h + 4; ++k) mma_bf16_a_tmem(d_o, a_p + k * 8, desc_v(dv + k * (2048 >> 4)), kIdescO, k > 0 ? 1u : more);
+            if (h) {
+              mma_commit(bar(C::kPv + t));
+              mma_commit(bar(C::kEmpty + st));
+            }
+          }
+          __syncwarp();
+        }
+        if (!C::kPlaceForP && ok && i + 1 < n) scores(i + 1);
+      }
+      if (!dual)                          // tiles that only the other query tile uses: free for this one, each once it is there
+        for (int c = 2 * n; c < 2 * copied && ok; ++c)
+          if (wait(C::kFull + (ring + c) % C::kStages, (ring + c) / C::kStages) && lane == 0) mbar_arrive(bar(C::kEmpty + (ring + c) % C::kStages));
+      steps += n;
       ring += 2 * copied;
       taken(k);
       if (!ok) break;
@@ -434,26 +469,38 @@ attention_packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
       for (int c = 0; c < p.copied; ++c) {
         const int slot = ring + 2 * c + 1, st = slot % C::kStages, key0 = (p.j0 + c) * BN, lo = p.lo, hi = p.hi;
         if (!wait(C::kFull + st, slot / C::kStages)) break;
-        uint8_t* v_tile = smem + 2 * C::kTile + st * C::kTile;
-        // warp 10 the first 64 rows, warp 11 the others; a lane the same piece of every fourth row
-#pragma unroll 8
-        for (int i = 0; i < (on_edge(p, c) ? 16 * C::kHalves : 0); ++i) {
-          const int r = (warp - kLookWarp) * 64 + (i & 15) * 4 + (lane >> 3), key = key0 + r;
-          uint4* at = reinterpret_cast<uint4*>(v_tile + (i >> 4) * C::kBlock + swz(r, lane & 7));
-          uint4 w = *at;
-          if (key < lo || key >= hi) {
-            *at = make_uint4(0, 0, 0, 0);
-          } else if (any_not_finite(w)) {
-            uint32_t* e = &w.x;
-            for (int q = 0; q < 4; ++q) {
-              if ((e[q] & 0x7f80u) == 0x7f80u) e[q] &= 0xffff0000u;
-              if ((e[q] & 0x7f800000u) == 0x7f800000u) e[q] &= 0xffffu;
+        uint8_t* v_tile = smem + C::kRing + st * C::kTile;
+        if (on_edge(p, c)) {
+          // a lane the same piece of every fourth row, eight rows at a time
+          auto at = [&](int i) { return reinterpret_cast<uint4*>(v_tile + (i >> 5) * C::kBlock + swz((i & 31) * 4 + (lane >> 3), lane & 7)); };
+#pragma unroll 1
+          for (int i0 = 0; i0 < 32 * C::kHalves; i0 += 8) {
+            uint4 w[8];
+            __nv_bfloat162 acc = __floats2bfloat162_rn(0.f, 0.f);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int key = key0 + ((i0 + i) & 31) * 4 + (lane >> 3);
+              w[i] = *at(i0 + i);
+              if (key < lo || key >= hi) *at(i0 + i) = w[i] = make_uint4(0, 0, 0, 0);
             }
-            *at = w;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) gather_not_finite(acc, w[i]);
+            if (__low2float(acc) == 0.f && __high2float(acc) == 0.f) continue;
+#pragma unroll 1
+            for (int i = i0; i < i0 + 8; ++i) {
+              uint4 x = *at(i);
+              uint32_t* e = &x.x;
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                if ((e[q] & 0x7f80u) == 0x7f80u) e[q] &= 0xffff0000u;
+                if ((e[q] & 0x7f800000u) == 0x7f800000u) e[q] &= 0xffffu;
+              }
+              *at(i) = x;
+            }
             *reinterpret_cast<volatile int*>(&p.bad) = 1;
           }
+          fence_async_proxy();
         }
-        fence_async_proxy();
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(C::kClean + st));
       }
@@ -534,6 +581,12 @@ attention_packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
           const Two scale2(a.scale_log2), minus2(m_ref == -INFINITY ? 0.f : -m_ref);
           Two sum2[2] = {Two(0.f), Two(0.f)};
           if (C::kPlaceForP && g > 0 && !wait(C::kPv + t, g - 1)) break;      // the tile before's P has been used
+          // The two warps of a scheduler that make exponentials do so one after the other where they can: the first is done in half the time,
+          // and its products run while the second is at it.  (No more than a hint: the wait ends by itself.)
+          if (!C::kPlaceForP) {
+            for (int polls = 0; s_turn[warp ^ 4] && polls < 64; ++polls) {}
+            s_turn[warp] = 1;
+          }
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             uint32_t packed[BN / 4];
@@ -548,18 +601,23 @@ attention_packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
               packed[c] = *reinterpret_cast<const uint32_t*>(&b);
             }
             tmem_st32(t_p + 32 * h, reinterpret_cast<const float*>(packed));
+            if (h == 1 && !C::kPlaceForP) s_turn[warp] = 0;
+            tmem_st_wait();
+            fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(C::kP + 2 * h + t));
           }
           float x, y;
           (sum2[0] + sum2[1]).get(x, y);
           l += x + y;
-          tmem_st_wait();
-        } else if (C::kPlaceForP) {
-          if (lane == 0) mbar_arrive(bar(C::kRead + t));
-          if (g > 0 && !wait(C::kPv + t, g - 1)) break;                       // (its arrival below must not count for the step before)
+        } else {
+          if (C::kPlaceForP) {
+            if (lane == 0) mbar_arrive(bar(C::kRead + t));
+            if (g > 0 && !wait(C::kPv + t, g - 1)) break;                     // (its arrivals below must not count for the step before)
+          }
+          __syncwarp();
+          if (lane == 0) { mbar_arrive(bar(C::kP + t)); mbar_arrive(bar(C::kP + 2 + t)); }
         }
-        fence_before_sync();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar(C::kP + t));
       }
       steps += n;
       if (n > 0) wait(C::kPv + t, steps - 1);
@@ -646,7 +704,7 @@ attention_packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
     if (warp == kCopyWarp && lane == 0) {
       for (int n = max(0, copies - C::kStages); n < copies; ++n) mbar_wait(bar(C::kFull + n % C::kStages), (n / C::kStages) & 1);
       for (int t = 0; t < 2; ++t)
-        if (copies_q[t] > 0) mbar_wait(bar(C::kQ + t), (copies_q[t] - 1) & 1);
+        for (int n = max(0, copies_q[t] - C::kSets); n < copies_q[t]; ++n) mbar_wait(bar(C::kQ + 2 * (n % C::kSets) + t), (n / C::kSets) & 1);
     }
     if (tid == 0) report(a.status, kGaveUp);
     __syncthreads();
@@ -684,6 +742,7 @@ int launch_one(const PackedArgs& a, const CUtensorMap& mq, const CUtensorMap& mk
       return fail(ERB_ERR_CUDA, "%s: built with too few registers for its split", who);
     configured[dev] = true;
   }
+  if (pieces > 0x7f000000LL) return fail(ERB_ERR_UNSUPPORTED, "%s: too many rows", who);
   launch_chained(attention_packed_tc_kernel<D, MODE>, dim3((unsigned)(pieces < sm_count() ? pieces : sm_count())), dim3(kThreads), Cfg<D>::kSmemBytes, stream,
                  mq, mk, mv, a, dual);
   return check_launch(who);
