@@ -331,9 +331,5 @@ ERB_EXPORT int erb_attention_shared_prefix(const void* q, long long ld_q, const 
   a.pieces = own_pieces;
   const int rc = launch_by_size<kOwn>(a, dim3((unsigned)(n_seqs * own_pieces), nkv, 1), s, "attention_shared_prefix");
   if (rc || n_rec <= 1) return rc;
-  const long long blocks = ((long long)n_tokens * nq + 3) / 4;
-  if (blocks > 0x7fffffffLL) return fail(ERB_ERR_UNSUPPORTED, "attention_shared_prefix: too many rows");
-  launch_chained(attention_merge_kernel, dim3((unsigned)blocks), dim3(128), 0, s, (const float*)part_o, (const float*)part_ml, (elem_t*)out, ld_out,
-                 seq_starts, n_seqs, n_tokens, nq, head_dim, n_rec);
-  return check_launch("attention_shared_prefix");
+  return launch_merge(a, s, "attention_shared_prefix");
 }

@@ -115,6 +115,13 @@ __device__ __forceinline__ bool wait_long(uint32_t bar, uint32_t parity, volatil
   return false;
 }
 
+// The largest of three, NaN if one of them is.
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
   asm volatile(
       "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
@@ -556,12 +563,13 @@ attention_packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
           }
           float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int c = 0; c < BN; ++c) m4[c & 3] = fmaxf(m4[c & 3], s[c]);
-          const float m_tile = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * a.scale_log2;
-          const bool move = m_tile > m_ref + kMoveFrom;
+          for (int c = 0; c < BN; c += 2) m4[(c >> 1) & 3] = max3_nan(m4[(c >> 1) & 3], s[c], s[c + 1]);
+          const float m_tile = max3_nan(max3_nan(m4[0], m4[1], m4[2]), m4[3], m4[3]) * a.scale_log2;
+          const bool move = !(m_tile <= m_ref + kMoveFrom);
           if (__any_sync(0xffffffffu, move)) {
-            const float alpha = move ? fast_exp2(m_ref - m_tile) : 1.f;       // 0 on the first tile
-            if (move) m_ref = m_tile;
+            // (0 on the first tile.  A row with a score that is no number, or infinite, becomes NaN as a whole.)
+            const float alpha = move ? fast_exp2(m_ref - m_tile) : 1.f;
+            if (move) m_ref = m_tile < INFINITY ? m_tile : NAN;
             l *= alpha;
             if (i > 0) {
               if (!wait(C::kPv + t, g - 1)) break;
@@ -850,9 +858,5 @@ ERB_EXPORT int erb_attention_shared_prefix_tc(const void* q, long long ld_q, con
     rc = head_dim == 64 ? launch_few<64>(a, own == kOwnToken, prefix_len > 0, s, who) : launch_few<128>(a, own == kOwnToken, prefix_len > 0, s, who);
     if (rc || own_pieces == 1) return rc;
   }
-  const long long blocks = ((long long)n_tokens * nq + 3) / 4;
-  if (blocks > 0x7fffffffLL) return fail(ERB_ERR_UNSUPPORTED, "%s: too many rows", who);
-  launch_chained(attention_merge_kernel, dim3((unsigned)blocks), dim3(128), 0, s, (const float*)part_o, (const float*)part_ml, (elem_t*)out, ld_out,
-                 seq_starts, n_seqs, n_tokens, nq, head_dim, n_rec);
-  return check_launch(who);
+  return launch_merge(a, s, who);
 }

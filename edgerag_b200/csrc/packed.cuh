@@ -93,7 +93,53 @@ __device__ __forceinline__ void key_rows(const PackedArgs& a, const int* table, 
   }
 }
 
-// Joins the records of each (token, head), in their order: a warp each.
+// Joins the n records (at most 128) of a row, in their order; the whole warp, lane l with the entries l + 32 c.  o starts at the row's
+// own unnormalised values with maximum m and sum l (l 0: none) and ends as the result.
+template <int C>
+__device__ __forceinline__ void join_records(const float* part_ml, const float* part_o, int n, int D, float m, float l, float* o) {
+  const int lane = threadIdx.x & 31;
+  float rm[4], rl[4], top = l != 0.f ? m : -INFINITY;
+#pragma unroll
+  for (int h = 0; h < 4; ++h) {
+    const int r = lane + 32 * h;
+    const float2 ml = r < n ? __ldcg(reinterpret_cast<const float2*>(part_ml) + r) : make_float2(-INFINITY, 0.f);
+    rm[h] = ml.x;
+    rl[h] = ml.y;
+    if (rl[h] != 0.f) top = fmaxf(top, rm[h]);
+  }
+  top = warp_max(top);
+  float sum = 0.f;
+#pragma unroll
+  for (int h = 0; h < 4; ++h) {
+    rm[h] = rl[h] != 0.f ? exp2f(rm[h] - top) : 0.f;             // the records' weights
+    sum = fmaf(rl[h], rm[h], sum);
+  }
+  const float mine = l != 0.f ? exp2f(m - top) : 0.f;
+  sum = fmaf(l, mine, warp_sum(sum));
+#pragma unroll
+  for (int c = 0; c < C; ++c) o[c] = l != 0.f ? o[c] * mine : 0.f;
+  for (int r0 = 0; r0 < n; r0 += 8) {                            // eight records' values on their way
+    float x[8][C];
+#pragma unroll
+    for (int r = 0; r < 8; ++r)
+#pragma unroll
+      for (int c = 0; c < C; ++c) x[r][c] = r0 + r < n && lane + 32 * c < D ? __ldcg(part_o + (size_t)(r0 + r) * D + lane + 32 * c) : 0.f;
+    const int h = r0 >> 5;
+    const float w8 = h == 0 ? rm[0] : h == 1 ? rm[1] : h == 2 ? rm[2] : rm[3], l8 = h == 0 ? rl[0] : h == 1 ? rl[1] : h == 2 ? rl[2] : rl[3];
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      const float w = __shfl_sync(0xffffffffu, w8, (r0 + r) & 31), lr = __shfl_sync(0xffffffffu, l8, (r0 + r) & 31);
+#pragma unroll
+      for (int c = 0; c < C; ++c) o[c] = lr != 0.f ? fmaf(x[r][c], w, o[c]) : o[c];      // (a record without a sum has no values)
+    }
+  }
+  const float inv = sum != 0.f ? 1.f / sum : 0.f;                // (a row that sees no key: zeros)
+#pragma unroll
+  for (int c = 0; c < C; ++c) o[c] *= inv;
+}
+
+// Joins the records of each (token, head): a warp each.
+template <int C>
 static __global__ void __launch_bounds__(128)
 attention_merge_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml, elem_t* __restrict__ out, long long ld_out,
                        const int* __restrict__ seq_starts, int n_seqs, int n_tokens, int nq, int D, int n_rec) {
@@ -102,27 +148,23 @@ attention_merge_kernel(const float* __restrict__ part_o, const float* __restrict
   const int lane = threadIdx.x & 31;
   const long long first = seq_starts[0], end = min((long long)seq_starts[n_seqs], (long long)n_tokens);
   if (first < 0 || item < first * nq || item >= end * nq) return;
-  const float* ml = part_ml + 2 * item * n_rec;
-  float m = -INFINITY;
-  for (int r = lane; r < n_rec; r += 32)
-    if (ml[2 * r + 1] != 0.f) m = fmaxf(m, ml[2 * r]);
-  m = warp_max(m);
-  float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, l = 0.f;
-  for (int r = 0; r < n_rec; ++r) {
-    const float sum = ml[2 * r + 1];
-    if (sum == 0.f) continue;
-    const float w = exp2f(ml[2 * r] - m);
-    l = fmaf(sum, w, l);
-    const float* src = part_o + (item * n_rec + r) * D;
+  float o[C];
 #pragma unroll
-    for (int c = 0; c < 8; ++c)
-      if (lane + 32 * c < D) o[c] = fmaf(src[lane + 32 * c], w, o[c]);
-  }
-  const float inv = l != 0.f ? 1.f / l : 0.f;
+  for (int c = 0; c < C; ++c) o[c] = 0.f;
+  join_records<C>(part_ml + 2 * item * n_rec, part_o + item * n_rec * D, n_rec, D, 0.f, 0.f, o);
   elem_t* dst = out + (item / nq) * ld_out + (item % nq) * D;
 #pragma unroll
-  for (int c = 0; c < 8; ++c)
-    if (lane + 32 * c < D) Elem<elem_t>::store(dst + lane + 32 * c, o[c] * inv);
+  for (int c = 0; c < C; ++c)
+    if (lane + 32 * c < D) Elem<elem_t>::store(dst + lane + 32 * c, o[c]);
+}
+
+static int launch_merge(const PackedArgs& a, cudaStream_t stream, const char* who) {
+  const long long blocks = ((long long)a.n_tokens * a.nq + 3) / 4;
+  if (blocks > 0x7fffffffLL) return fail(ERB_ERR_UNSUPPORTED, "%s: too many rows", who);
+  auto kern = a.D <= 64 ? attention_merge_kernel<2> : a.D <= 128 ? attention_merge_kernel<4> : attention_merge_kernel<8>;
+  launch_chained(kern, dim3((unsigned)blocks), dim3(128), 0, stream, (const float*)a.part_o, (const float*)a.part_ml, a.out, a.ld_out, a.seq_starts, a.n_seqs,
+                 a.n_tokens, a.nq, a.D, a.n_rec);
+  return check_launch(who);
 }
 
 }  // namespace erb

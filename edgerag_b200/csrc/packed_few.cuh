@@ -140,11 +140,11 @@ __device__ __forceinline__ void few_fetch(const PackedArgs& a, uint32_t k_tile, 
   }
 }
 
-// One row's result: this block's m, l and (unnormalised) o, lane `lane` with D / 32 neighbouring entries, joined with the records of the
-// prefix where the block is the last to add to it, else left as a record.
+// One row's result: this block's m, l and (unnormalised) o, lane l with the entries l + 32 c, joined with the records of the prefix where
+// the block is the last to add to it, else left as a record.
 template <int D>
 __device__ __forceinline__ void few_result(const PackedArgs& a, int token, int head, int piece, bool final, float m, float l, float* o) {
-  constexpr int E = D / 32;
+  constexpr int C = D / 32;
   const int lane = threadIdx.x & 31;
   const size_t row = (size_t)token * a.nq + head;
   if (!final) {
@@ -152,45 +152,13 @@ __device__ __forceinline__ void few_result(const PackedArgs& a, int token, int h
     if (lane == 0) { a.part_ml[2 * record] = m; a.part_ml[2 * record + 1] = l; }
     if (l == 0.f) return;
 #pragma unroll
-    for (int e = 0; e < E; e += 2) *reinterpret_cast<float2*>(a.part_o + record * D + lane * E + e) = make_float2(o[e], o[e + 1]);
+    for (int c = 0; c < C; ++c) a.part_o[record * D + lane + 32 * c] = o[c];
     return;
   }
-  const int n = a.rec0;                                   // records of the prefix (at most 64)
-  float rm[2], rl[2], top = l != 0.f ? m : -INFINITY;
+  join_records<C>(a.part_ml + 2 * row * a.n_rec, a.part_o + row * a.n_rec * D, a.rec0, D, m, l, o);
+  elem_t* dst = a.out + (long long)token * a.ld_out + (long long)head * D;
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int r = lane + 32 * h;
-    const float2 ml = r < n ? __ldcg(reinterpret_cast<const float2*>(a.part_ml) + row * a.n_rec + r) : make_float2(-INFINITY, 0.f);
-    rm[h] = ml.x;
-    rl[h] = ml.y;
-    if (rl[h] != 0.f) top = fmaxf(top, rm[h]);
-  }
-  top = warp_max(top);
-  const float mine = l != 0.f ? fast_exp2(m - top) : 0.f;
-  float w[2];
-#pragma unroll
-  for (int h = 0; h < 2; ++h) w[h] = rl[h] != 0.f ? fast_exp2(rm[h] - top) : 0.f;
-  const float sum = warp_sum(rl[0] * w[0] + rl[1] * w[1]) + l * mine;
-#pragma unroll
-  for (int e = 0; e < E; ++e) o[e] = l != 0.f ? o[e] * mine : 0.f;
-  const float* src = a.part_o + row * a.n_rec * D + lane * E;
-#pragma unroll 4
-  for (int r = 0; r < n; ++r) {
-    const float wr = __shfl_sync(0xffffffffu, r < 32 ? w[0] : w[1], r & 31), lr = __shfl_sync(0xffffffffu, r < 32 ? rl[0] : rl[1], r & 31);
-    float x[E];
-#pragma unroll
-    for (int e = 0; e < E; e += 2) {
-      const float2 two = __ldcg(reinterpret_cast<const float2*>(src + (size_t)r * D + e));
-      x[e] = two.x;
-      x[e + 1] = two.y;
-    }
-#pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = lr != 0.f ? fmaf(x[e], wr, o[e]) : o[e];      // (a record without a sum has no values)
-  }
-  const float inv = sum != 0.f ? 1.f / sum : 0.f;
-  elem_t* dst = a.out + (long long)token * a.ld_out + (long long)head * D + lane * E;
-#pragma unroll
-  for (int e = 0; e < E; e += 2) *reinterpret_cast<__nv_bfloat162*>(dst + e) = __floats2bfloat162_rn(o[e] * inv, o[e + 1] * inv);
+  for (int c = 0; c < C; ++c) dst[lane + 32 * c] = __float2bfloat16_rn(o[c]);
 }
 
 template <int D> struct FewSmem {
@@ -288,7 +256,7 @@ __global__ void __launch_bounds__(kFewThreads) attention_own_token_kernel(const 
         const float f = fast_exp2(joint_ml[(w * 16 + r) * 2] - m);
         l = fmaf(lw, f, l);
 #pragma unroll
-        for (int e = 0; e < E; ++e) o[e] = fmaf(joint[(w * 16 + r) * D + lane * E + e], f, o[e]);
+        for (int e = 0; e < E; ++e) o[e] = fmaf(joint[(w * 16 + r) * D + lane + 32 * e], f, o[e]);
       }
       few_result<D>(a, token, kvh * G + r, piece, final, m, l, o);
     }
@@ -442,7 +410,7 @@ __global__ void __launch_bounds__(kFewThreads) attention_own_rows_kernel(const P
     const float m = __shfl_sync(0xffffffffu, r < 8 ? rows.m[0] : rows.m[1], from_lane), l = __shfl_sync(0xffffffffu, r < 8 ? rows.l[0] : rows.l[1], from_lane);
     float o[E];
 #pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = mine[r * D + lane * E + e];
+    for (int e = 0; e < E; ++e) o[e] = mine[r * D + lane + 32 * e];
     const int index = r0 + 16 * warp + r;
     few_result<D>(a, t0 + index / G, kvh * G + index % G, piece, final, m, l, o);
   }
