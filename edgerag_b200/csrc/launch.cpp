@@ -182,6 +182,55 @@ PyObject* need(PyObject*, PyObject* const* args, Py_ssize_t n, PyObject* kwnames
   return PyObject_Vectorcall(g_need, args, (size_t)n, kwnames);
 }
 
+// rows(tensor, rows, width, dtype, written): the stride between the rows of heads [rows, width] where they are as an entry point takes them
+// (inner stride 1; rows that are written do not overlap), else None: the check in Python words what is wrong.
+PyObject* rows(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n == 5 && THPVariable_Check(args[0]) && PyLong_Check(args[1]) && PyLong_Check(args[2]) && THPDtype_Check(args[3])) {
+    const at::Tensor& t = THPVariable_Unpack(args[0]);
+    const long long many = PyLong_AsLongLong(args[1]), width = PyLong_AsLongLong(args[2]);
+    try {
+      if (t.scalar_type() == reinterpret_cast<THPDtype*>(args[3])->scalar_type && t.dim() == 2 && t.size(0) == many && t.size(1) == width &&
+          (t.stride(1) == 1 || width <= 1) && (args[4] != Py_True || many <= 1 || t.stride(0) >= width))
+        return PyLong_FromLongLong(many > 1 ? t.stride(0) : width);
+    } catch (const std::exception&) {                          // (as in need)
+    }
+  }
+  PyErr_Clear();
+  Py_RETURN_NONE;
+}
+
+// vector(tensor, dtype, entries): whether it is contiguous, of that type, and has at least so many entries.
+PyObject* vector(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  bool good = false;
+  if (n == 3 && THPVariable_Check(args[0]) && THPDtype_Check(args[1]) && PyLong_Check(args[2])) {
+    const at::Tensor& t = THPVariable_Unpack(args[0]);
+    try {
+      good = t.scalar_type() == reinterpret_cast<THPDtype*>(args[1])->scalar_type && t.numel() >= PyLong_AsLongLong(args[2]) && t.is_contiguous();
+    } catch (const std::exception&) {
+    }
+  }
+  PyErr_Clear();
+  return PyBool_FromLong(good);
+}
+
+// here(device, tensors..): whether every tensor (None aside) is on that CUDA device.
+PyObject* here(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  const long device = n ? PyLong_AsLong(args[0]) : -1;
+  bool good = device >= 0;
+  for (Py_ssize_t i = 1; i < n && good; ++i) {
+    if (args[i] == Py_None) continue;
+    good = false;
+    if (!THPVariable_Check(args[i])) break;
+    const at::Tensor& t = THPVariable_Unpack(args[i]);
+    try {
+      good = t.is_cuda() && t.get_device() == device;
+    } catch (const std::exception&) {
+    }
+  }
+  PyErr_Clear();
+  return PyBool_FromLong(good);
+}
+
 // bind(counts, KernelError, the check in Python)
 PyObject* bind(PyObject*, PyObject* args) {
   PyObject *counts, *error, *check;
@@ -198,6 +247,9 @@ PyMethodDef methods[] = {
     {"launcher", make_launcher, METH_VARARGS, nullptr},
     {"bind", bind, METH_VARARGS, nullptr},
     {"call", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(checked_call)), METH_FASTCALL, nullptr},
+    {"rows", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(rows)), METH_FASTCALL, nullptr},
+    {"vector", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(vector)), METH_FASTCALL, nullptr},
+    {"here", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(here)), METH_FASTCALL, nullptr},
     {"need", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(need)), METH_FASTCALL | METH_KEYWORDS, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };

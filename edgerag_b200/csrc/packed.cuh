@@ -98,15 +98,24 @@ __device__ __forceinline__ void key_rows(const PackedArgs& a, const int* table, 
 template <int C>
 __device__ __forceinline__ void join_records(const float* part_ml, const float* part_o, int n, int D, float m, float l, float* o) {
   const int lane = threadIdx.x & 31;
-  float rm[4], rl[4], top = l != 0.f ? m : -INFINITY;
+  float rm[4], rl[4], x[8][C], top = l != 0.f ? m : -INFINITY;
+  auto values = [&](int r0) {                                    // of eight records, on their way at once
+#pragma unroll
+    for (int r = 0; r < 8; ++r)
+#pragma unroll
+      for (int c = 0; c < C; ++c) x[r][c] = r0 + r < n && lane + 32 * c < D ? __ldcg(part_o + (size_t)(r0 + r) * D + lane + 32 * c) : 0.f;
+  };
 #pragma unroll
   for (int h = 0; h < 4; ++h) {
     const int r = lane + 32 * h;
     const float2 ml = r < n ? __ldcg(reinterpret_cast<const float2*>(part_ml) + r) : make_float2(-INFINITY, 0.f);
     rm[h] = ml.x;
     rl[h] = ml.y;
-    if (rl[h] != 0.f) top = fmaxf(top, rm[h]);
   }
+  values(0);
+#pragma unroll
+  for (int h = 0; h < 4; ++h)
+    if (rl[h] != 0.f) top = fmaxf(top, rm[h]);
   top = warp_max(top);
   float sum = 0.f;
 #pragma unroll
@@ -118,12 +127,8 @@ __device__ __forceinline__ void join_records(const float* part_ml, const float* 
   sum = fmaf(l, mine, warp_sum(sum));
 #pragma unroll
   for (int c = 0; c < C; ++c) o[c] = l != 0.f ? o[c] * mine : 0.f;
-  for (int r0 = 0; r0 < n; r0 += 8) {                            // eight records' values on their way
-    float x[8][C];
-#pragma unroll
-    for (int r = 0; r < 8; ++r)
-#pragma unroll
-      for (int c = 0; c < C; ++c) x[r][c] = r0 + r < n && lane + 32 * c < D ? __ldcg(part_o + (size_t)(r0 + r) * D + lane + 32 * c) : 0.f;
+  for (int r0 = 0; r0 < n; r0 += 8) {
+    if (r0) values(r0);
     const int h = r0 >> 5;
     const float w8 = h == 0 ? rm[0] : h == 1 ? rm[1] : h == 2 ? rm[2] : rm[3], l8 = h == 0 ? rl[0] : h == 1 ? rl[1] : h == 2 ? rl[2] : rl[3];
 #pragma unroll

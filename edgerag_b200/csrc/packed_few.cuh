@@ -113,28 +113,28 @@ template <int D> struct FewRows {
   }
 };
 
-// The first element of key `key`'s row in the pools, or -1 where nothing is to be fetched.
-__device__ __forceinline__ long long few_row(const PackedArgs& a, const int* table, int kvh, int key, int hi) {
+// The page of key `key`, and with it the key's row in the pools, or -1 where nothing is to be fetched.  The page may be
+// asked for before it is known whether the request has the key.  (Rows of a pool are counted in 32 bits: the launch looks.)
+__device__ __forceinline__ int few_page(const PackedArgs& a, const int* table, int key) { return __ldcg(table + min(key / a.page_size, a.table_ld - 1)); }
+__device__ __forceinline__ int few_row(const PackedArgs& a, int page, int kvh, int key, int hi) {
   if (key >= hi) return -1;
-  const int page = __ldcg(table + key / a.page_size);
   if (page < 0 || page >= a.n_pages) {
     report(a.status, kBadPage);
     return -1;
   }
-  return (((long long)page * a.nkv + kvh) * a.page_size + key % a.page_size) * a.D;
+  return (page * a.nkv + kvh) * a.page_size + key % a.page_size;
 }
 
 // A warp's ask for 16 keys and values; lane r (and r + 16) holds key r's place.
 template <int D>
-__device__ __forceinline__ void few_fetch(const PackedArgs& a, uint32_t k_tile, uint32_t v_tile, long long place) {
+__device__ __forceinline__ void few_fetch(const PackedArgs& a, uint32_t k_tile, uint32_t v_tile, int place) {
   constexpr int PIECES = D / 8, AT_ONCE = 32 / PIECES;
   const int lane = threadIdx.x & 31, c = lane % PIECES;
 #pragma unroll
   for (int r0 = 0; r0 < 16; r0 += AT_ONCE) {
-    const int r = r0 + lane / PIECES;
-    const long long row = __shfl_sync(0xffffffffu, place, r);
+    const int r = r0 + lane / PIECES, row = __shfl_sync(0xffffffffu, place, r);
     const bool valid = row >= 0;
-    const long long from = valid ? row + c * 8 : 0;
+    const long long from = (long long)max(row, 0) * D + c * 8;
     cp_async16(k_tile + few_at<D>(r, c), a.k + from, valid);
     cp_async16(v_tile + few_at<D>(r, c), a.v + from, valid);
   }
@@ -161,23 +161,29 @@ __device__ __forceinline__ void few_result(const PackedArgs& a, int token, int h
   for (int c = 0; c < C; ++c) dst[lane + 32 * c] = __float2bfloat16_rn(o[c]);
 }
 
+// Two stages: blocks are short (a request's few hundred keys), so four of them on a multiprocessor hide more than a deep ring would.
 template <int D> struct FewSmem {
-  static constexpr int kStages = D == 64 ? 4 : 3;
+  static constexpr int kStages = 2;
   static constexpr uint32_t kTile = 16 * D * 2;                                 // 16 keys or values
-  static constexpr uint32_t kBytes = kFewWarps * kStages * 2 * kTile;           // both forms: 16 keys a stage and warp, or 64 in all and 32 a stage
+  static constexpr uint32_t kRing = kFewWarps * kStages * 2 * kTile, kJoint = kFewWarps * 16 * (D + 2) * 4;
+  static constexpr uint32_t kBytes = kRing > kJoint ? kRing : kJoint;           // (the warps' results lie over their rings)
 };
 
 template <int D>
-__global__ void __launch_bounds__(kFewThreads) attention_own_token_kernel(const PackedArgs a, const int early) {
+__global__ void __launch_bounds__(kFewThreads, D == 64 ? 4 : 3) attention_own_token_kernel(const PackedArgs a, const int early) {
   using S = FewSmem<D>;
   extern __shared__ __align__(128) uint8_t few_smem[];
   if (!early) chain_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = a.nq / a.nkv, kvh = blockIdx.x, seq = blockIdx.y, piece = blockIdx.z;
+  // Asked for at once: the request's rows, its first keys' pages, and the position of its row where every request has one.
+  const int* table = a.tables + (size_t)seq * a.table_ld;
+  const long long from = (long long)a.prefix_len + (long long)piece * a.piece_keys;
+  const int lo = (int)min(from, (long long)INT_MAX - 4096);
+  const int page_first = few_page(a, table, lo + 16 * warp + (lane & 15)), position_guess = __ldcg(a.positions + min(seq, a.n_tokens - 1));
   const int t0 = __ldcg(a.seq_starts + seq), len = __ldcg(a.seq_starts + seq + 1) - t0;
   const bool bad = len > 0 && (t0 < 0 || t0 + (long long)len > a.n_tokens);
   if (bad && threadIdx.x == 0) report(a.status, kBadStarts);
   const bool final = a.n_rec == a.rec0 + 1;
-  const int* table = a.tables + (size_t)seq * a.table_ld;
   const uint32_t mine = smem_u32(few_smem) + warp * S::kStages * 2 * S::kTile;
   float* joint = reinterpret_cast<float*>(few_smem);                            // [warp][16 rows][D], then [warp][16][2]
   float* joint_ml = joint + kFewWarps * 16 * D;
@@ -185,23 +191,23 @@ __global__ void __launch_bounds__(kFewThreads) attention_own_token_kernel(const 
   bool waited = !early;
   for (int i = 0; i < (bad ? 0 : len); ++i) {
     const int token = t0 + i;
-    long long limit = (long long)__ldcg(a.positions + token) + 1;
+    long long limit = (long long)(token == seq ? position_guess : __ldcg(a.positions + token)) + 1;
     if (limit > (long long)a.table_ld * a.page_size) {
       if (threadIdx.x == 0) report(a.status, kBadPage);
       limit = (long long)a.table_ld * a.page_size;
     }
-    const long long from = (long long)a.prefix_len + (long long)piece * a.piece_keys;
-    const int lo = (int)min(from, (long long)INT_MAX), hi = (int)(piece + 1 < a.pieces ? min(limit, from + a.piece_keys) : limit);
+    const int hi = (int)(piece + 1 < a.pieces ? min(limit, from + a.piece_keys) : limit);
     // this warp's chunks: 16 keys from lo + 16 (warp + 4 c) on
     const int n = hi > lo ? ((hi - lo + 15) / 16 - warp + kFewWarps - 1) / kFewWarps : 0;
     auto key_of = [&](int c) { return lo + 16 * (warp + kFewWarps * c); };
-    auto place_of = [&](int c) { return c < n ? few_row(a, table, kvh, key_of(c) + (lane & 15), hi) : -1; };
-    long long place = place_of(0);
+    auto page_of = [&](int c) { return c == 0 ? page_first : c < n ? few_page(a, table, key_of(c) + (lane & 15)) : -1; };
+    auto place_of = [&](int c, int page) { return c < n ? few_row(a, page, kvh, key_of(c) + (lane & 15), hi) : -1; };
+    int page = page_of(0);
 #pragma unroll
     for (int c = 0; c < S::kStages - 1; ++c) {
-      if (c < n) few_fetch<D>(a, mine + c * 2 * S::kTile, mine + (c * 2 + 1) * S::kTile, place);
+      if (c < n) few_fetch<D>(a, mine + c * 2 * S::kTile, mine + (c * 2 + 1) * S::kTile, place_of(c, page));
       cp_async_commit();
-      place = place_of(c + 1);
+      page = page_of(c + 1);
     }
     const int g = lane >> 2;
     const elem_t* q = a.q + (long long)token * a.ld_q + (long long)kvh * G * D;
@@ -215,10 +221,10 @@ __global__ void __launch_bounds__(kFewThreads) attention_own_token_kernel(const 
       const int next = c + S::kStages - 1;
       if (next < n) {
         const uint32_t dst = mine + (next % S::kStages) * 2 * S::kTile;
-        few_fetch<D>(a, dst, dst + S::kTile, place);
+        few_fetch<D>(a, dst, dst + S::kTile, place_of(next, page));
       }
       cp_async_commit();
-      place = place_of(next + 1);
+      page = page_of(next + 1);
     }
     cp_async_wait<0>();
     rows.sum_lanes();
@@ -321,8 +327,11 @@ __global__ void __launch_bounds__(kFewThreads) attention_own_rows_kernel(const P
   const int n = hi > lo ? (hi - lo + S::kKeys - 1) / S::kKeys : 0, least = s_min;
   // warp w fetches keys 16 (w & 1) .. of a stage, warps 0 and 1 their keys, 2 and 3 their values
   const uint32_t ring = smem_u32(few_smem);
-  auto place_of = [&](int c) { return c < n ? few_row(a, table, kvh, lo + S::kKeys * c + 16 * (warp & 1) + (lane & 15), hi) : -1; };
-  auto fetch = [&](int c, long long place) {
+  auto place_of = [&](int c) {
+    const int key = lo + S::kKeys * c + 16 * (warp & 1) + (lane & 15);
+    return c < n && key < hi ? few_row(a, few_page(a, table, key), kvh, key, hi) : -1;
+  };
+  auto fetch = [&](int c, int place) {
     constexpr int PIECES = D / 8, AT_ONCE = 32 / PIECES;
     const elem_t* pool = warp >= 2 ? a.v : a.k;
     const uint32_t dst = ring + (c % S::kStages) * 2 * S::kTile + (warp >= 2 ? S::kTile : 0);
@@ -330,11 +339,11 @@ __global__ void __launch_bounds__(kFewThreads) attention_own_rows_kernel(const P
 #pragma unroll
     for (int r1 = 0; r1 < 16; r1 += AT_ONCE) {
       const int r = r1 + lane / PIECES;
-      const long long row = __shfl_sync(0xffffffffu, place, r);
-      cp_async16(dst + few_at<D>(16 * (warp & 1) + r, p), pool + (row >= 0 ? row + p * 8 : 0), row >= 0);
+      const int row = __shfl_sync(0xffffffffu, place, r);
+      cp_async16(dst + few_at<D>(16 * (warp & 1) + r, p), pool + (long long)max(row, 0) * D + p * 8, row >= 0);
     }
   };
-  long long place = place_of(0);
+  int place = place_of(0);
 #pragma unroll
   for (int c = 0; c < S::kStages - 1; ++c) {
     if (c < n) fetch(c, place);

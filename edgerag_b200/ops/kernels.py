@@ -2285,26 +2285,36 @@ def attention_prefill_tc(qkv: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
 
 def _packed_rows(t: torch.Tensor, name: str, who: str, rows: int, width: int, dtype: torch.dtype, written: bool = False) -> int:
     """Checks rows of heads (inner stride 1, any stride between rows); their stride."""
-    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != width or t.dtype != dtype:
+    if _host:
+        stride = _host.rows(t, rows, width, dtype, written)
+        if stride is not None:
+            return stride
+    if t.dtype is not dtype or t.shape != (rows, width):
         raise KernelError(f"{who}: {name} must be [{rows}, {width}] of {dtype}, got {list(t.shape)} of {t.dtype}")
-    if (width > 1 and t.stride(1) != 1) or (written and rows > 1 and t.stride(0) < width):
+    between, inside = t.stride()
+    if (inside != 1 and width > 1) or (written and rows > 1 and between < width):
         raise KernelError(f"{who}: rows of {name} must be contiguous" + (" and may not overlap" if written else ""))
-    return t.stride(0) if rows > 1 else width
+    return between if rows > 1 else width
 
 
 def _packed_vector(t: torch.Tensor | None, name: str, who: str, dtype: torch.dtype, at_least: int) -> None:
-    if t is None or t.dtype != dtype or t.numel() < at_least or not t.is_contiguous():
+    if _host and _host.vector(t, dtype, at_least):
+        return
+    if t is None or t.dtype is not dtype or t.numel() < at_least or not t.is_contiguous():
         raise KernelError(f"{who}: {name} must be contiguous {dtype} with at least {at_least} entries")
 
 
-def _on_this_device(who: str, **tensors) -> None:
+def _on_this_device(who: str, *tensors: torch.Tensor | None) -> None:
     """Every tensor on the current CUDA device: that is where the launch goes."""
-    for name, t in tensors.items():
-        if t is None:
-            continue
-        _need(t, name, contiguous=False)
-        if t.get_device() != torch._C._cuda_getDevice():
-            raise KernelError(f"{who}: {name} is on {t.device}, the current device is cuda:{torch._C._cuda_getDevice()}")
+    if _host and tensors[0].is_cuda and _host.here(torch._C._cuda_getDevice(), *tensors):
+        return
+    for t in tensors:
+        if t is not None and not t.is_cuda:
+            raise KernelError(f"{who}: a tensor is not on a CUDA device")
+    here = torch._C._cuda_getDevice()
+    for t in tensors:
+        if t is not None and t.get_device() != here:
+            raise KernelError(f"{who}: a tensor is on {t.device}, the current device is cuda:{here}")
 
 
 _INVERSE_TURN = Fraction("0.159154943091895335768883763372514362034459645740456448747667344")       # 1 / (2 pi)
@@ -2381,8 +2391,7 @@ def rotary_append(q: torch.Tensor, positions: torch.Tensor, turns: torch.Tensor 
         if n:
             _packed_vector(slots, "slots", who, torch.int32, n)
         _packed_vector(status, "status", who, torch.int32, 1)
-    _on_this_device(who, q=q, q_out=q_out, k=k, k_out=k_out, v=v, positions=positions, turns=turns, q_norm=q_norm, k_norm=k_norm, slots=slots,
-                    k_pages=k_pages, v_pages=v_pages, status=status)
+    _on_this_device(who, q, q_out, k, k_out, v, positions, turns, q_norm, k_norm, slots, k_pages, v_pages, status)
     if n == 0:
         return
     _call(_fn("rotary", _elem(q), "erb_rotary_append"), q, q if q_out is None else q_out, ld_q, ld_qo, k,
@@ -2405,8 +2414,12 @@ def packed_tc_supported(dtype: torch.dtype, head_dim: int, group: int, page_size
     return dtype == torch.bfloat16 and head_dim in (64, 128) and group <= 128 and 8 <= page_size <= 128 and page_size & (page_size - 1) == 0
 
 
-def _on_16_bytes(*tensors: torch.Tensor) -> bool:
-    return all(t.data_ptr() % 16 == 0 and (t.dim() != 2 or t.shape[0] <= 1 or t.stride(0) * t.element_size() % 16 == 0) for t in tensors)
+def _on_16_bytes(strides: int, *tensors: torch.Tensor) -> bool:
+    """Whether bfloat16 tensors start, and their rows (the strides' common bits) lie, on 16-byte boundaries."""
+    for t in tensors:
+        if t.data_ptr() & 15:
+            return False
+    return strides & 7 == 0
 
 
 def attention_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seq_starts: torch.Tensor, out: torch.Tensor, n_q_heads: int,
@@ -2430,10 +2443,10 @@ def attention_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seq_star
     _packed_vector(status, "status", who, torch.int32, 1)
     if n * (n_q_heads // n_kv_heads) >= 1 << 30:
         raise KernelError(f"{who}: {n} tokens of {n_q_heads} heads in one call")
-    _on_this_device(who, q=q, k=k, v=v, seq_starts=seq_starts, out=out, status=status)
+    _on_this_device(who, q, k, v, seq_starts, out, status)
     if n == 0 or seq_starts.numel() == 1:
         return
-    if packed_tc_supported(q.dtype, head_dim, n_q_heads // n_kv_heads) and _on_16_bytes(q, k, v, out) and min(ld_k, ld_v) >= n_kv_heads * head_dim:
+    if packed_tc_supported(q.dtype, head_dim, n_q_heads // n_kv_heads) and _on_16_bytes(ld_q | ld_k | ld_v | ld_o, q, k, v, out) and min(ld_k, ld_v) >= n_kv_heads * head_dim:
         fn = _fn("attention_packed_tc", None, "erb_attention_prompt_tc")
     else:
         fn = _fn("attention_packed", _elem(q), "erb_attention_prompt")
@@ -2492,8 +2505,7 @@ def shared_prefix_plan(n_tokens: int, n_seqs: int, n_q_heads: int, n_kv_heads: i
             blocks = n_kv_heads * max(1, n_seqs if own == OWN_TOKEN else -(-n_tokens * group // 64))
             cut = min(max(1, 4 * sms // blocks), max(1, own_keys // 512), 64)
             piece_keys = -(-own_keys // (64 * cut)) * 64
-            tiles = -(-own_keys // 128)
-        own_pieces = max(1, -(-tiles * 128 // piece_keys))
+        own_pieces = max(1, -(-(tiles * 128 if own == OWN_MANY else own_keys) // piece_keys))
         records = prefix_pieces + own_pieces
         return SharedPrefixPlan(prefix_pieces, own_pieces, piece_keys, n_tokens * n_q_heads * records * (head_dim + 2) if records > 1 else 0, True,
                                 prefix_dual, own)
@@ -2551,12 +2563,11 @@ def attention_shared_prefix(q: torch.Tensor, k_pages: torch.Tensor, v_pages: tor
         raise KernelError(f"{who}: the plan does not fit a prefix of {prefix_len} keys")
     floats = n * n_q_heads * records * head_dim if records > 1 else 0
     _packed_vector(scratch, "scratch", who, torch.float32, floats + (n * n_q_heads * records * 2 if records > 1 else 0))
-    _on_this_device(who, q=q, k_pages=k_pages, v_pages=v_pages, prefix_pages=prefix_pages, block_tables=block_tables, seq_starts=seq_starts,
-                    positions=positions, out=out, scratch=scratch, status=status)
+    _on_this_device(who, q, k_pages, v_pages, prefix_pages, block_tables, seq_starts, positions, out, scratch, status)
     if n == 0 or n_seqs == 0:
         return
     part_o = scratch.data_ptr()
-    if plan.tensor_cores and packed_tc_supported(q.dtype, head_dim, n_q_heads // n_kv_heads, page_size) and _on_16_bytes(q, out, k_pages, v_pages, scratch) \
+    if plan.tensor_cores and packed_tc_supported(q.dtype, head_dim, n_q_heads // n_kv_heads, page_size) and _on_16_bytes(ld_q | ld_o, q, out, k_pages, v_pages, scratch) \
             and n_pages * n_kv_heads * page_size <= 0x7fffffff:
         fn, how = _fn("attention_packed_tc", None, "erb_attention_shared_prefix_tc"), (int(plan.prefix_dual), plan.own)
     else:
