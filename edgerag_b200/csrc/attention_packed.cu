@@ -20,16 +20,35 @@ namespace {
 
 constexpr int BM = 64, BN = 64, kThreads = 256;
 
+// Floats on 16-byte boundaries are copied asynchronously, the next keys while these are worked on: two places for keys and values where
+// two blocks still fit a multiprocessor (heads up to 64) or one does (128).
 template <int DMAX> struct Smem {
-  static constexpr int kLd = DMAX + 4, kLdP = BN + 4;
-  float q[BM * kLd], k[BN * kLd], v[BN * DMAX], p[BM * kLdP];
+  static constexpr int kLd = DMAX + 4, kLdP = BN + 4, kBufs = sizeof(elem_t) == 4 && DMAX <= 128 ? 2 : 1;
+  float q[BM * kLd], k[kBufs][BN * kLd], v[kBufs][BN * DMAX], p[BM * kLdP];
   int limit[BM], any[2];
-  const elem_t* krow[BN];
-  const elem_t* vrow[BN];
+  const elem_t* krow[kBufs][BN];
+  const elem_t* vrow[kBufs][BN];
 };
 
+// Four entries from column c on of a row as floats, zeros behind column D; `wide`: rows lie on four entries' boundaries.
+__device__ __forceinline__ float4 load_four(const elem_t* row, int c, int D, bool wide) {
+  float x[4] = {0.f, 0.f, 0.f, 0.f};
+  if (wide) {
+    if (c < D) Pack4<elem_t>::load(row + c, x);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (c + j < D) x[j] = Elem<elem_t>::load(row + c + j);
+  }
+  return make_float4(x[0], x[1], x[2], x[3]);
+}
+__device__ __forceinline__ void copy16(float* dst, const void* src, bool real) {
+  const uint32_t d = (uint32_t)__cvta_generic_to_shared(dst);
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(src), "r"(real ? 16 : 0) : "memory");
+}
+
 template <int DMAX, int MODE>
-__global__ void __launch_bounds__(kThreads) attention_packed_kernel(const PackedArgs a) {
+__global__ void __launch_bounds__(kThreads) attention_packed_kernel(const PackedArgs a, const int wide) {
   chain_wait();
   extern __shared__ __align__(16) uint8_t raw[];
   Smem<DMAX>& sm = *reinterpret_cast<Smem<DMAX>*>(raw);
@@ -77,16 +96,12 @@ __global__ void __launch_bounds__(kThreads) attention_packed_kernel(const Packed
       sm.limit[tid] = lim;
       atomicMax(&sm.any[0], lim);
     }
+#pragma unroll 4
     for (int i = tid; i < BM * (DMAX / 4); i += kThreads) {
       const int r = i / (DMAX / 4), c = (i % (DMAX / 4)) * 4;
-      float x[4] = {0.f, 0.f, 0.f, 0.f};
-      if (r < rows) {
-        const elem_t* src = a.q + (long long)(t0 + (r0 + r) / G) * a.ld_q + (long long)(kvh * G + (r0 + r) % G) * D + c;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (c + j < D) x[j] = Elem<elem_t>::load(src + j) * a.scale_log2;
-      }
-      *reinterpret_cast<float4*>(sm.q + r * LD + c) = make_float4(x[0], x[1], x[2], x[3]);
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (r < rows) x = load_four(a.q + (long long)(t0 + (r0 + r) / G) * a.ld_q + (long long)(kvh * G + (r0 + r) % G) * D, c, D, wide);
+      *reinterpret_cast<float4*>(sm.q + r * LD + c) = make_float4(x.x * a.scale_log2, x.y * a.scale_log2, x.z * a.scale_log2, x.w * a.scale_log2);
     }
     __syncthreads();
     // the keys of this block's piece, [lo, hi)
@@ -110,31 +125,59 @@ __global__ void __launch_bounds__(kThreads) attention_packed_kernel(const Packed
 #pragma unroll
       for (int c = 0; c < 4 * NC; ++c) o[i][c] = 0.f;
     }
-    for (int key0 = lo; key0 < hi; key0 += BN) {
-      __syncthreads();
+    constexpr int BUFS = Smem<DMAX>::kBufs;
+    const bool async = BUFS == 2 && wide;
+    auto find_rows = [&](int key0, int buf) {
       if (tid < BN) {
         const elem_t *kr = nullptr, *vr = nullptr;
         if (key0 + tid < hi) key_rows<MODE>(a, table, t0, kvh, key0 + tid, kr, vr);
-        sm.krow[tid] = kr;
-        sm.vrow[tid] = vr;
+        sm.krow[buf][tid] = kr;
+        sm.vrow[buf][tid] = vr;
       }
+    };
+    auto fetch = [&](int buf) {                    // the rows found, asynchronously
+      constexpr int N = BN * (DMAX / 4) / kThreads;
+#pragma unroll 4
+      for (int n = 0; n < N; ++n) {
+        const int i = tid + n * kThreads, r = i / (DMAX / 4), c = (i % (DMAX / 4)) * 4;
+        const elem_t *kr = sm.krow[buf][r], *vr = sm.vrow[buf][r];
+        const bool real = kr && c < D;
+        copy16(sm.k[buf] + r * LD + c, real ? kr + c : a.k, real);
+        copy16(sm.v[buf] + r * DMAX + c, real ? vr + c : a.v, real);
+      }
+    };
+    int buf = 0;
+    if (async && lo < hi) {
+      find_rows(lo, 0);
       __syncthreads();
-      for (int i = tid; i < BN * (DMAX / 4); i += kThreads) {
-        const int r = i / (DMAX / 4), c = (i % (DMAX / 4)) * 4;
-        float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
-        const elem_t *kr = sm.krow[r], *vr = sm.vrow[r];
-        if (kr) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (c + j < D) {
-              x[j] = Elem<elem_t>::load(kr + c + j);
-              y[j] = Elem<elem_t>::load(vr + c + j);
-            }
+      fetch(0);
+    }
+    if (async) asm volatile("cp.async.commit_group;" ::: "memory");
+    for (int key0 = lo; key0 < hi; key0 += BN) {
+      if (async) {
+        buf = ((key0 - lo) / BN) & 1;
+        __syncthreads();                           // (the other place has been left)
+        find_rows(key0 + BN, buf ^ 1);
+        __syncthreads();
+        if (key0 + BN < hi) fetch(buf ^ 1);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
+        __syncthreads();
+      } else {
+        __syncthreads();
+        find_rows(key0, 0);
+        __syncthreads();
+#pragma unroll 4
+        for (int i = tid; i < BN * (DMAX / 4); i += kThreads) {
+          const int r = i / (DMAX / 4), c = (i % (DMAX / 4)) * 4;
+          const elem_t *kr = sm.krow[0][r], *vr = sm.vrow[0][r];
+          const float4 none = make_float4(0.f, 0.f, 0.f, 0.f);
+          *reinterpret_cast<float4*>(sm.k[0] + r * LD + c) = kr ? load_four(kr, c, D, wide) : none;
+          *reinterpret_cast<float4*>(sm.v[0] + r * DMAX + c) = kr ? load_four(vr, c, D, wide) : none;
         }
-        *reinterpret_cast<float4*>(sm.k + r * LD + c) = make_float4(x[0], x[1], x[2], x[3]);
-        *reinterpret_cast<float4*>(sm.v + r * DMAX + c) = make_float4(y[0], y[1], y[2], y[3]);
+        __syncthreads();
       }
-      __syncthreads();
+      const float *tile_k = sm.k[buf], *tile_v = sm.v[buf];
       // scores: rows ty + 16 i, keys tx + 16 j
       float s[4][4];
 #pragma unroll
@@ -146,7 +189,7 @@ __global__ void __launch_bounds__(kThreads) attention_packed_kernel(const Packed
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           qa[i] = *reinterpret_cast<const float4*>(sm.q + (ty + 16 * i) * LD + c);
-          ka[i] = *reinterpret_cast<const float4*>(sm.k + (tx + 16 * i) * LD + c);
+          ka[i] = *reinterpret_cast<const float4*>(tile_k + (tx + 16 * i) * LD + c);
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -193,7 +236,7 @@ __global__ void __launch_bounds__(kThreads) attention_packed_kernel(const Packed
           for (int jj = 0; jj < 4; ++jj)
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
-              const float4 va = *reinterpret_cast<const float4*>(sm.v + (j + jj) * DMAX + 64 * c + 4 * tx);
+              const float4 va = *reinterpret_cast<const float4*>(tile_v + (j + jj) * DMAX + 64 * c + 4 * tx);
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
                 const float p = jj == 0 ? pa[i].x : jj == 1 ? pa[i].y : jj == 2 ? pa[i].z : pa[i].w;
@@ -213,7 +256,7 @@ __global__ void __launch_bounds__(kThreads) attention_packed_kernel(const Packed
             const float p = sm.p[(ty + 16 * i) * LDP + j];
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
-              const float4 va = *reinterpret_cast<const float4*>(sm.v + j * DMAX + 64 * c + 4 * tx);
+              const float4 va = *reinterpret_cast<const float4*>(tile_v + j * DMAX + 64 * c + 4 * tx);
               o[i][4 * c] = fmaf(p, va.x, o[i][4 * c]);
               o[i][4 * c + 1] = fmaf(p, va.y, o[i][4 * c + 1]);
               o[i][4 * c + 2] = fmaf(p, va.z, o[i][4 * c + 2]);
@@ -265,7 +308,10 @@ int launch_tiles(const PackedArgs& a, dim3 grid, cudaStream_t stream, const char
     if (e != cudaSuccess) return fail(ERB_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
     configured[dev] = true;
   }
-  launch_chained(attention_packed_kernel<DMAX, MODE>, grid, dim3(kThreads), bytes, stream, a);
+  // whether every row starts on a boundary of four entries (floats: of 16 bytes)
+  const uintptr_t starts = (uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v;
+  const int wide = !(starts & (4 * sizeof(elem_t) - 1)) && !((a.ld_q | a.D | (MODE == kPrompt ? a.ld_k | a.ld_v : 0)) & 3);
+  launch_chained(attention_packed_kernel<DMAX, MODE>, grid, dim3(kThreads), bytes, stream, a, wide);
   return check_launch(who);
 }
 
