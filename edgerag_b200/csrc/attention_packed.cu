@@ -2,9 +2,10 @@
 // are: packed.cuh): the kernels on CUDA cores, for both element types, any head size up to 256, any page size, strides and alignment; and
 // the merge of the pieces that a call's keys were cut into.  attention_packed_tc.cu has the tensor-core forms.
 //
-// A block owns 64 rows of one kv head and walks its keys 64 at a time with the running maximum and sum of the softmax.  Queries, keys and
-// values lie in shared memory as floats; a thread of the 256 owns 4 x 4 scores and then 4 rows x D / 16 entries of the result, so that
-// 16 products take 8 floats from shared memory.  What bounds it: the fused multiply-adds of CUDA cores.
+// A block owns 32 rows of one kv head and walks its keys 64 at a time with the running maximum and sum of the softmax.  Queries, keys and
+// values lie in shared memory as floats; a thread of the 128 owns 4 x 4 scores and then 4 rows x D / 16 entries of the result, so that
+// 16 products take 8 floats from shared memory.  What bounds it: the fused multiply-adds of CUDA cores, and the
+// longest row tile's walk (5 prompts of up to 701 tokens, 15 heads of 64: tiles of 64 rows 113 us, of 32 84 us).
 //
 // Keys that no row of the block may see are zeros in shared memory, whatever their memory holds; where only some rows may see a key, its
 // product is left out for the others, not multiplied by zero, so that an infinity or NaN there stays unseen.
@@ -18,7 +19,7 @@ ERB_DEFINE_LAST_ERROR(erb_last_error)
 
 namespace {
 
-constexpr int BM = 64, BN = 64, kThreads = 256;
+constexpr int BM = 32, BN = 64, kThreads = 4 * BM, RS = BM / 4;      // (a thread's rows are RS apart)
 
 // Floats on 16-byte boundaries are copied asynchronously, the next keys while these are worked on: two places for keys and values where
 // two blocks still fit a multiprocessor (heads up to 64) or one does (128).
@@ -188,7 +189,7 @@ __global__ void __launch_bounds__(kThreads) attention_packed_kernel(const Packed
         float4 qa[4], ka[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          qa[i] = *reinterpret_cast<const float4*>(sm.q + (ty + 16 * i) * LD + c);
+          qa[i] = *reinterpret_cast<const float4*>(sm.q + (ty + RS * i) * LD + c);
           ka[i] = *reinterpret_cast<const float4*>(tile_k + (tx + 16 * i) * LD + c);
         }
 #pragma unroll
@@ -200,7 +201,7 @@ __global__ void __launch_bounds__(kThreads) attention_packed_kernel(const Packed
       bool partly = false;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int lim = min(sm.limit[ty + 16 * i], hi);
+        const int lim = min(sm.limit[ty + RS * i], hi);
         partly |= lim < key0 + BN;
         float top = -INFINITY;
 #pragma unroll
@@ -217,7 +218,7 @@ __global__ void __launch_bounds__(kThreads) attention_packed_kernel(const Packed
         for (int j = 0; j < 4; ++j) {
           const float p = exp2f(s[i][j] - base);
           sum += p;
-          sm.p[(ty + 16 * i) * LDP + tx + 16 * j] = p;
+          sm.p[(ty + RS * i) * LDP + tx + 16 * j] = p;
         }
 #pragma unroll
         for (int w = 8; w > 0; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
@@ -231,7 +232,7 @@ __global__ void __launch_bounds__(kThreads) attention_packed_kernel(const Packed
         for (int j = 0; j < BN; j += 4) {
           float4 pa[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) pa[i] = *reinterpret_cast<const float4*>(sm.p + (ty + 16 * i) * LDP + j);
+          for (int i = 0; i < 4; ++i) pa[i] = *reinterpret_cast<const float4*>(sm.p + (ty + RS * i) * LDP + j);
 #pragma unroll
           for (int jj = 0; jj < 4; ++jj)
 #pragma unroll
@@ -252,8 +253,8 @@ __global__ void __launch_bounds__(kThreads) attention_packed_kernel(const Packed
         for (int j = 0; j < n; ++j) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            if (key0 + j >= sm.limit[ty + 16 * i]) continue;
-            const float p = sm.p[(ty + 16 * i) * LDP + j];
+            if (key0 + j >= sm.limit[ty + RS * i]) continue;
+            const float p = sm.p[(ty + RS * i) * LDP + j];
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
               const float4 va = *reinterpret_cast<const float4*>(tile_v + j * DMAX + 64 * c + 4 * tx);
@@ -268,7 +269,7 @@ __global__ void __launch_bounds__(kThreads) attention_packed_kernel(const Packed
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int r = ty + 16 * i;
+      const int r = ty + RS * i;
       if (r >= rows) continue;
       const int token = t0 + (r0 + r) / G, head = kvh * G + (r0 + r) % G;
       if (direct) {

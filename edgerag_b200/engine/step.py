@@ -103,6 +103,8 @@ class StepContext:
         self.embeds: torch.Tensor | None = None
         self.max_pages = 1
         self.bound_pages, self.granule_pages = 4, 1
+        #: every portion of the step (entries of more than one token) is the beginning of its prompt
+        self.whole_portions = False
         self.graph_key: tuple | None = None          # set when the step has the fixed layout of a CUDA graph
         self.slots: list[torch.Tensor] = []
         self.block_tables: list[torch.Tensor] = []
@@ -375,12 +377,15 @@ class ModelRunner:
         ctx.block_tables = [tables_d[g * per: (g + 1) * per].view(n_seqs, max_pages) for g in range(n_groups)]
         ctx.n_tokens, ctx.n_seqs, ctx.n_decode, ctx.n_wanted = total, n_seqs, n_decode, int(want_rows.size)
         ctx.n_wanted_real = n_wanted_real
+        ctx.whole_portions = all(self.cache.requests[e.request_id].num_tokens == 0 for e in ordered[n_decode - n_fill:])
         ctx.max_pages = max_pages
         ctx.bound_pages, ctx.granule_pages = bound_pages, granule_pages
         ctx.n_fed_back = sum(1 for e in ordered if e.fed_back is not None)
         if graphable:
             ctx.graph_key = (n_decode, tuple(e.n_tokens for e in ordered[n_decode - n_fill:]), max_pages, bound_pages,
                              int(want_rows.size))
+            if getattr(self.model, "whole_prompts", False):
+                ctx.graph_key += (ctx.whole_portions,)
         if embed_chunks:
             ctx.embeds = torch.cat([c.to(device=self.device, dtype=self.dtype, non_blocking=True)
                                     for c in embed_chunks], dim=0).contiguous()
@@ -429,7 +434,8 @@ class ModelRunner:
             if code >= 1000000:
                 raise StepError(f"an attention kernel gave up (code {code}: 1xxxxxx prefill wait, 2xxxxxx decode wait, 3000000 shared-memory "
                                 "alignment, 4xxxxxx a wait of a product for few rows, 5xxxxxx of the experts' products, 7000000 of the "
-                                "state-space chunks, 8000000 of the delta rule's); the step's results are not valid")
+                                "state-space chunks, 8000000 of the delta rule's, 9000001 a page or position outside the cache, 9000002 sequences "
+                                "outside the rows, 9100000 a wait of attention over packed requests); the step's results are not valid")
             raise StepError(f"a kernel flagged token {code - 1} of the batch (id or row out of range)")
 
     def drop_graphs(self) -> None:

@@ -61,6 +61,8 @@ class DecoderModel:
             getattr(getattr(b.mixer, "position", None), "graph_safe", True) for b in self.blocks)
         #: some part looks at the tokens' ids: rows of embeddings cannot stand in for them
         self.needs_token_ids = any(part.needs_token_ids for _, part in self._owners)
+        #: some mixer takes prompts that begin in a step from its rows: what a captured step does then depends on that, too
+        self.whole_prompts = any(getattr(b.mixer, "whole_prompts", False) for b in self.blocks)
         limits = [part.max_positions for _, part in self._owners if part.max_positions is not None]
         #: positions that some part has no row for start here (None: no such part)
         self.max_positions = min(limits) if limits else None

@@ -2511,7 +2511,7 @@ def shared_prefix_plan(n_tokens: int, n_seqs: int, n_q_heads: int, n_kv_heads: i
                                 prefix_dual, own)
     # Two blocks a multiprocessor, tiles of 64 keys, two tiles a piece at least.
     rows = n_tokens * (n_q_heads // n_kv_heads)
-    blocks = max(1, -(-rows // 64) * n_kv_heads)
+    blocks = max(1, -(-rows // 32) * n_kv_heads)
     tiles = -(-prefix_len // 64)
     prefix_pieces = min(max(1, 2 * sms // blocks), max(1, tiles // 2), 64) if prefix_len else 0
     own_pieces = min(max(1, 2 * sms // max(1, n_seqs * n_kv_heads)), max(1, own_keys // 128), 64)

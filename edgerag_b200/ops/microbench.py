@@ -5,6 +5,7 @@
     python -m edgerag_b200.ops.microbench linear --m 8 --n 6144 --k 2048
     python -m edgerag_b200.ops.microbench latent-attention --batch 8 --context 8192
     python -m edgerag_b200.ops.microbench ssm-scan --batch 8 --tokens 1
+    python -m edgerag_b200.ops.microbench packed-ops --tokens 8192 --batch 64 --prefix 16384
     python -m edgerag_b200.ops.microbench step-kernels --layers 4 --batch 8 --context 8192 --iters 4
 
 Each case builds random inputs larger than the 126 MB L2 where the real workload is (or says that
@@ -755,6 +756,47 @@ def input_ops(a) -> dict:
     return res
 
 
+def packed_ops(a) -> dict:
+    """Rows turned and appended, packed prompts, and a batch behind a shared prefix, each against its bytes and operations."""
+    dtype = torch.bfloat16 if a.dtype == "bfloat16" else torch.float32
+    nq, nkv, d, size = a.heads, a.kv_heads, a.head_dim, 2 if a.dtype == "bfloat16" else 4
+    n, status = a.tokens, torch.zeros(1, dtype=torch.int32, device="cuda")
+    rows = lambda *shape: torch.randn(shape, device="cuda").to(dtype)      # noqa: E731
+    qkv, out = rows(n, (nq + 2 * nkv) * d), torch.empty((n, nq * d), device="cuda", dtype=dtype)
+    q, k, v = qkv[:, : nq * d], qkv[:, nq * d: (nq + nkv) * d], qkv[:, (nq + nkv) * d:]
+    scale, record = d ** -0.5, {"case": "packed-ops", "heads": nq, "kv_heads": nkv, "head_dim": d, "dtype": a.dtype}
+
+    kp, vp, tables = _paged(1, n, nkv, d, a.page, dtype)
+    at = torch.arange(n, device="cuda")
+    slots = (tables[0].long()[at // a.page] * a.page + at % a.page).to(torch.int32)
+    turns = kernels.rotary_turns(10000.0 ** (-torch.arange(d // 2, dtype=torch.float64) / (d // 2))).cuda()
+    positions = at.to(torch.int32)
+    us = _time(lambda: kernels.rotary_append(q, positions, turns, nq, nkv, d, k=k, v=v, q_out=out, slots=slots, k_pages=kp, v_pages=vp, status=status),
+               a.iters, a.warmup)
+    nbytes = 2 * n * (nq + 2 * nkv) * d * size
+    record["rotary_append"] = {"tokens": n, "us": round(us, 2), "gbs": round(nbytes / us / 1e3, 1), "frac_hbm": round(nbytes / us / 1e3 / HBM_GBS, 4)}
+
+    starts = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+    us = _time(lambda: kernels.attention_prompt(q, k, v, starts, out, nq, nkv, scale, status), a.iters, a.warmup)
+    flops = 4 * d * nq * n * (n + 1) / 2
+    record["attention_prompt"] = {"tokens": n, "us": round(us, 2), "tflops": round(flops / us / 1e6, 1), "frac_bf16": round(flops / us / 1e6 / BF16_TFLOPS, 4)}
+
+    b, prefix, own = a.batch, a.prefix, a.own
+    shared, mine = -(-prefix // a.page), -(-(prefix + own) // a.page) - prefix // a.page
+    kp, vp = rows(shared + b * mine, nkv, a.page, d), rows(shared + b * mine, nkv, a.page, d)
+    order = torch.randperm(shared + b * mine, device="cuda").to(torch.int32)
+    tables = torch.cat((order[: prefix // a.page].expand(b, -1), order[shared:].view(b, mine)), 1).contiguous()
+    plan = kernels.shared_prefix_plan(b, b, nq, nkv, d, dtype, a.page, prefix, prefix + own)
+    scratch, qb, ob = torch.empty(max(plan.floats, 1), device="cuda"), rows(b, nq * d), torch.empty((b, nq * d), device="cuda", dtype=dtype)
+    seq, pos = torch.arange(b + 1, dtype=torch.int32, device="cuda"), torch.full((b,), prefix + own - 1, dtype=torch.int32, device="cuda")
+    us = _time(lambda: kernels.attention_shared_prefix(qb, kp, vp, order[:shared], prefix, tables, seq, pos, ob, nq, scale, plan, scratch, status), a.iters, a.warmup)
+    nbytes = 2 * ((prefix + b * own) * nkv + b * nq) * d * size
+    record["attention_shared_prefix"] = {"batch": b, "prefix": prefix, "own": own, "us": round(us, 2), "gbs": round(nbytes / us / 1e3, 1),
+                                         "frac_hbm": round(nbytes / us / 1e3 / HBM_GBS, 4)}
+    record["status"] = int(status)
+    return record
+
+
 def main(argv=None) -> int:
     ap = argparse.ArgumentParser(prog="edgerag_b200.ops.microbench", description=__doc__.split("\n\n")[0])
     sub = ap.add_subparsers(dest="case", required=True)
@@ -877,13 +919,22 @@ def main(argv=None) -> int:
     io.add_argument("--width", type=int, default=2048)
     io.add_argument("--heads", type=int, default=32)
     io.add_argument("--kv-heads", type=int, default=8)
+    po = sub.add_parser("packed-ops", parents=[common])
+    po.add_argument("--tokens", type=int, default=2048, help="tokens of the rows that are turned, and of the prompt")
+    po.add_argument("--heads", type=int, default=32)
+    po.add_argument("--kv-heads", type=int, default=8)
+    po.add_argument("--head-dim", type=int, default=128)
+    po.add_argument("--page", type=int, default=16)
+    po.add_argument("--batch", type=int, default=64, help="requests behind the shared prefix, one new token each")
+    po.add_argument("--prefix", type=int, default=16384)
+    po.add_argument("--own", type=int, default=256, help="keys of each request behind the prefix")
     a = ap.parse_args(argv)
     if not torch.cuda.is_available():
         print("microbench needs a CUDA device", file=sys.stderr)
         return 1
     fn = {"decode-attention": decode_attention, "prefill-attention": prefill_attention, "linear": linear,
           "step-kernels": step_kernels, "step-timeline": step_timeline, "latent-attention": latent_attention,
-          "ssm-scan": ssm_scan, "delta-scan": delta_scan, "routed-experts": routed_experts, "diff-attention": diff_attention, "stream-ops": stream_ops, "input-ops": input_ops}[a.case]
+          "ssm-scan": ssm_scan, "delta-scan": delta_scan, "routed-experts": routed_experts, "diff-attention": diff_attention, "stream-ops": stream_ops, "input-ops": input_ops, "packed-ops": packed_ops}[a.case]
     load_peaks(a.peaks)
     result = fn(a)
     result["peaks"] = PEAKS_FROM

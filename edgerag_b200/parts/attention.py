@@ -33,6 +33,11 @@ multiply as they write); ``value_mix`` (``"first"``: the layer leaves its values
 values are ``(1 - l) v + l v'`` with the values ``v'`` that the ``"first"`` layer made of the same tokens and ``l`` the one number of the
 tensor ``vmix``).
 
+With positions scaled for long contexts (``rope_scaled``) the norm per head, the rotation and the cache write are one kernel
+(``kernels.rotary_append``).  ``whole_prompts``: where every portion of a step is its prompt's beginning, keys and values are taken from the step's
+rows instead of the cache (``kernels.attention_prompt``: tensor cores for heads of 64 and 128); positions then have to be scaled ones or none,
+since only those leave the rows' keys as the cache has them.
+
 Heads whose sizes differ or are no multiple of 8 are stored padded with zeros to one size ``D``:
 scores and outputs are unchanged, and the norm's mean divides by the true count.
 
@@ -48,6 +53,7 @@ import torch
 from ..cache.manager import KVGroupSpec, StateSpec
 from ..ops import kernels
 from .base import LayerCall, Mixer, PartSpec, WeightSpec, build_part, register_part
+from .rope import RotaryScaled
 
 
 @register_part("mixer", "attention")
@@ -60,7 +66,7 @@ class Attention(Mixer):
                  values_are_keys: bool = False, names: dict[str, str] | None = None, chunk: int = 0, v_dim: int | None = None,
                  all_bias: bool = False, whole_norm_eps: float | None = None, qkv_bias: bool = False, conv: int = 0,
                  penalty: tuple[str, str] | None = None, softcap: float = 0.0, gate: str | None = None,
-                 value_mix: str | None = None, vmix: str = "vmix") -> None:
+                 value_mix: str | None = None, vmix: str = "vmix", whole_prompts: bool = False) -> None:
         if n_q_heads % n_kv_heads:
             raise ValueError(f"{n_q_heads} query heads are not divisible by {n_kv_heads} kv heads")
         self.chunk = int(chunk or 0)
@@ -107,6 +113,16 @@ class Attention(Mixer):
         self.scale = float(head_dim ** -0.5 if scale is None else scale)
         self.dtype, self.device = dtype, device
         self.position = build_part("position", position, dtype, device)
+        #: positions scaled for long contexts: their kernel also norms the heads and writes the cache
+        self.scaled = isinstance(self.position, RotaryScaled)
+        if self.scaled and (self.whole or self.qk_bias or self.values_are_keys):
+            raise ValueError("attention: scaled positions go with a norm per head, not with biases, shared values or the second family of options")
+        self.whole_prompts = bool(whole_prompts)
+        if self.whole_prompts and (not (self.scaled or position.kind == "none") or self.whole or not own_kv or self.window or self.chunk
+                                   or self.values_are_keys or self.qk_bias or penalty or self.softcap
+                                   or (qk_norm_eps is not None and not self.scaled)):
+            raise ValueError("attention: whole prompts are taken from their rows: keys of the layer's own, positions scaled or none, and no other option "
+                             "than a norm per head with scaled positions")
         self.q_width = n_q_heads * head_dim
         self.kv_width = n_kv_heads * head_dim
         self.in_width = self.q_width + (1 if self.values_are_keys else 2) * self.kv_width
@@ -243,6 +259,11 @@ class Attention(Mixer):
                                    v_pages=None if pages is None else pages[1], page_size=ctx.page_size, first_values=first,
                                    blend=self.blend)
             return
+        if self.scaled:
+            kernels.linear(x, self.w_qkv, qkv)
+            self.position.prepare(qkv, ctx, self.n_q, self.n_kv, d, pages, slots, self.q_norm, self.k_norm, self.qk_norm_eps or 0.0,
+                                  keys_stay=self.whole_prompts and ctx.whole_portions and ctx.n_tokens > ctx.n_decode)
+            return
         if self.qk_bias or self.qk_norm_eps is not None or self.values_are_keys:
             pos = self.position
             kernels.linear(x, self.w_qkv, qkv)
@@ -334,7 +355,10 @@ class Attention(Mixer):
                                          out_rows, self.n_q, self.scale, part_acc, part_ml, max_splits,
                                          window=self.window, split_keys=split, keep_first=self.keep_first, chunk=self.chunk,
                                          gate=head_gate, **score)
-        if n > nd and kernels.prefill_tc_supported(self.dtype, d, self.window, ctx.page_size):
+        if n > nd and self.whole_prompts and ctx.whole_portions:        # keys and values are all in the step's rows
+            q, k, v = qkv[:, : self.q_width], qkv[:, self.q_width: self.q_width + self.kv_width], qkv[:, self.q_width + self.kv_width:]
+            kernels.attention_prompt(q, k, v, ctx.seq_starts[nd:], out, self.n_q, self.n_kv, self.scale, ctx.status)
+        elif n > nd and kernels.prefill_tc_supported(self.dtype, d, self.window, ctx.page_size):
             blocks = kernels.prefill_tc_blocks(ctx.host_q_len[nd:])
             # a portion that is short against its past: its few blocks' keys are cut into ranges
             reach = ctx.max_keys_bound()

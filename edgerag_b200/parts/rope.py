@@ -10,6 +10,9 @@ the same kernel that writes keys and values to their cache slots, so the cache h
 ``position * theta**(-2i / rot_dim) / factor`` (``factor``: linear scaling of positions) and leaves the rest
 of the head as it is.
 
+``RotaryScaled`` turns either kind of pairs by frequencies that are scaled for long contexts, with angles that stay right at any position
+(the two above round ``position * frequency`` to 32 bits: 0.06 radians at position 10^6).
+
 ``NoPosition`` encodes nothing and only writes the cache; it is what a mixer uses when another
 part has already put positions into the stream.
 """
@@ -118,6 +121,38 @@ class RotaryPairs(PositionEncoding):
         k_pages, v_pages = pages if pages is not None else (None, None)
         kernels.qk_prepare(qkv, ctx.positions, n_q_heads, n_kv_heads, head_dim, inv_freq=self.inv_freq, rot_dim=self.rot_dim,
                            pairs=True, slots=slots, k_pages=k_pages, v_pages=v_pages, page_size=ctx.page_size)
+
+
+@register_part("position", "rope_scaled")
+class RotaryScaled(PositionEncoding):
+    """Neighbouring pairs (``pairs``) or halves of the first ``rot_dim`` entries, turned by ``rotary_frequencies(theta, rot_dim, scaling)``, cosines
+    and sines times ``rotary_multiplier(scaling)``."""
+
+    graph_safe = True
+
+    def __init__(self, head_dim: int, theta: float, dtype: torch.dtype, device: torch.device, rot_dim: int | None = None,
+                 scaling: dict | None = None, pairs: bool = False) -> None:
+        self.head_dim, self.pairs = head_dim, bool(pairs)
+        self.rot_dim = head_dim if rot_dim is None else int(rot_dim)
+        if self.rot_dim % 2 or not 0 <= self.rot_dim <= head_dim:
+            raise ValueError(f"rot_dim {self.rot_dim} must be even and at most head_dim {head_dim}")
+        self.theta, self.multiplier = float(theta), rotary_multiplier(scaling)
+        self.turns = kernels.rotary_turns(rotary_frequencies(self.theta, self.rot_dim, scaling)).to(device)
+
+    def prepare(self, qkv, ctx, n_q_heads, n_kv_heads, head_dim, pages, slots, q_norm=None, k_norm=None, eps=0.0, keys_stay=False) -> None:
+        """What ``apply_and_store`` does, after a norm per head where weights are given; ``keys_stay``: the rows' keys are also rewritten."""
+        qw, kw = n_q_heads * head_dim, n_kv_heads * head_dim
+        q, k, v = qkv[:, :qw], qkv[:, qw: qw + kw], qkv[:, qw + kw: qw + 2 * kw]
+        if pages is None:                    # queries on another layer's keys
+            kernels.rotary_append(q, ctx.positions, self.turns, n_q_heads, n_kv_heads, head_dim, pairs=self.pairs, multiplier=self.multiplier,
+                                  q_norm=q_norm, eps=eps)
+            return
+        kernels.rotary_append(q, ctx.positions, self.turns, n_q_heads, n_kv_heads, head_dim, k=k, v=v, pairs=self.pairs,
+                              multiplier=self.multiplier, q_norm=q_norm, k_norm=k_norm, eps=eps, k_out=k if keys_stay else None, slots=slots,
+                              k_pages=pages[0], v_pages=pages[1], status=ctx.status)
+
+    def apply_and_store(self, qkv, ctx, n_q_heads, n_kv_heads, head_dim, pages, slots) -> None:
+        self.prepare(qkv, ctx, n_q_heads, n_kv_heads, head_dim, pages, slots)
 
 
 @register_part("position", "none")
