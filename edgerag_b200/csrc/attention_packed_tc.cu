@@ -13,17 +13,18 @@
 //   warp 10 (copy)      finds the pieces and describes them to the others; brings Q tiles, and K and V tiles in turn into one ring of
 //                       shared memory, by TMA tensor copies (128-byte swizzle): from the pages, one copy per page and 64 columns, or from
 //                       rows beside the queries
-//   warps 8, 9 (issue)  S_t = Q_t K^T (M 128, N 128) and O_t += P_t V (M 128, N D, P from TMEM), a warp for each query tile: a product
+//   warps 8, 9 (issue)  S_t = Q_t K^T (M 128, N 64) and O_t += P_t V (M 128, N D, K 64, P from TMEM), a warp for each query tile: a product
 //                       starts some 300 clocks after what it waits for, which one warp for both would leave the tensor cores idle
-//   warps 0-3, 4-7      softmax of tile A and of tile B: a thread owns a row, takes its 128 scores into registers, and writes P back
+//   warps 0-3, 4-7      softmax of tile A and of tile B: a thread owns a row, takes 64 of its scores into registers, and writes P back
 //                       rounded to bfloat16 (the second product's operand type; the sum of P is taken before that rounding, in float)
 //   warp 11 (look)      looks over the values of tiles with hidden keys (below)
 //
 // A row's reference maximum moves only when a tile's maximum is 2^8 above it; O is rescaled in TMEM then.  P is a floating-point number, so
 // a reference that is low by eight powers of two costs no precision.
 //
-// TMEM, 512 columns: S 2 x 128, O 2 x D.  With heads of 64 P has 2 x 64 columns of its own, so the next scores are issued as soon as a
-// tile's are in registers; with heads of 128 P takes its scores' place and the next scores wait for P V.
+// A tile's keys are worked on in two halves of 64, each with a place of its own for its scores in TMEM (512 columns: S 2 x 2 x 64, O 2 x D),
+// and P takes the place of the scores it was made of: the next tile's scores of a half are made behind P V of this tile's, while the softmax
+// is at the other half.
 //
 // Hidden keys.  Scores are masked where some row of a warp sees fewer keys than its tile has.  P is then zero, but zero times a value
 // that is no number would spoil rows that do not see it; so the values of such tiles are looked over before they are used: rows of V that
@@ -60,16 +61,15 @@ template <int D> struct Cfg {
   static constexpr uint32_t kBlock = BM * 128, kTile = kHalves * kBlock;
   static constexpr int kStages = D == 64 ? 8 : 4;                // tiles of K or V in the ring (a power of two)
   static constexpr int kSets = D == 64 ? 2 : 1;                  // pairs of Q tiles
-  static constexpr bool kPlaceForP = D == 64;
-  static constexpr uint32_t kColP = 256, kColO = D == 64 ? 384 : 256;
+  static constexpr uint32_t kColO = 256;
   static constexpr uint32_t kOutBytes = 2048;                    // a softmax warp's place for results on their way out: 32 rows of 64 bytes
   static_assert(kStages % 2 == 0, "a place of the ring holds keys or values, never both");
-  // barriers: ring full and empty; descriptions full and empty; a ring place's values looked over; per query tile: queries there and used, scores there,
-  // scores in registers, each half of P written, P V done
+  // barriers: ring full and empty; descriptions full and empty; a ring place's values looked over; per query tile: queries there and used;
+  // per query tile t and half u of a tile's keys, at + 2 u + t: scores there, P written, P V done
   static constexpr int kFull = 0, kEmpty = kStages, kTold = 2 * kStages, kTaken = kTold + kPieces, kClean = kTaken + kPieces, kQ = kClean + kStages,
-                       kQUsed = kQ + 2 * kSets, kS = kQUsed + 2 * kSets, kRead = kS + 2, kP = kS + 4, kPv = kS + 8, kNumBars = kS + 10;
+                       kQUsed = kQ + 2 * kSets, kS = kQUsed + 2 * kSets, kP = kS + 4, kPv = kS + 8, kNumBars = kS + 12;
   static constexpr uint32_t kRing = 2 * kSets * kTile, kSmemTiles = kRing + kStages * kTile, kSmemOut = kSmemTiles + kSoftmaxWarps * kOutBytes;
-  static constexpr uint32_t kSmemBytes = kSmemOut + 8 * kNumBars + 16 + kPieces * 64 + 32 + 1024;
+  static constexpr uint32_t kSmemBytes = kSmemOut + 8 * kNumBars + 16 + kPieces * 64 + 1024;
 };
 
 // A piece of work: rows r0 .. r0 + rows of the (token, head) pairs of the tokens from t0 on, key tiles j0 .. j0 + copied.
@@ -195,7 +195,6 @@ attention_packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(smem + C::kSmemOut + 8 * C::kNumBars + 8);
   auto bar = [&](int which) { return bars + 8u * (uint32_t)which; };
   auto piece_at = [&](int k) { return reinterpret_cast<Piece*>(smem + C::kSmemOut + 8 * C::kNumBars + 16 + (k % kPieces) * 64); };
-  volatile int* s_turn = reinterpret_cast<volatile int*>(smem + C::kSmemOut + 8 * C::kNumBars + 16 + kPieces * 64);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int G = a.nq / a.nkv, RT = BM / G * G, per_piece = dual ? RT : 2 * RT;      // rows of a query tile (whole tokens), of a piece
 
@@ -204,14 +203,13 @@ attention_packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
     for (int k = 0; k < kPieces; ++k) { mbar_init(bar(C::kTold + k), 1); mbar_init(bar(C::kTaken + k), kSoftmaxWarps + 3); }
     for (int t = 0; t < 2; ++t) {
       for (int s = 0; s < C::kSets; ++s) { mbar_init(bar(C::kQ + 2 * s + t), 1); mbar_init(bar(C::kQUsed + 2 * s + t), dual ? 2 : 1); }
-      mbar_init(bar(C::kS + t), 1);
-      mbar_init(bar(C::kRead + t), 4);
-      mbar_init(bar(C::kP + t), 4);
-      mbar_init(bar(C::kP + 2 + t), 4);
-      mbar_init(bar(C::kPv + t), 1);
+      for (int u = 0; u < 2; ++u) {
+        mbar_init(bar(C::kS + 2 * u + t), 1);
+        mbar_init(bar(C::kP + 2 * u + t), 4);
+        mbar_init(bar(C::kPv + 2 * u + t), 1);
+      }
     }
     *s_abort = 0;
-    for (int w = 0; w < kSoftmaxWarps; ++w) s_turn[w] = 0;
     mbar_init_fence();
   }
   if (warp == kIssueWarp) {
@@ -399,7 +397,7 @@ attention_packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
     const bool elected = elect_one();
     auto uniform = [](uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); };
     const uint32_t tm = uniform(tmem);
-    constexpr uint32_t kIdescS = mma_idesc(BM, BN, false), kIdescO = mma_idesc(BM, D, true);
+    constexpr uint32_t kIdescS = mma_idesc(BM, BN / 2, false), kIdescO = mma_idesc(BM, D, true);
     const uint64_t like = make_desc(0);                        // a descriptor without its address, which is the low 14 bits
     const uint32_t dq0 = uniform(sQ >> 4), dk0 = uniform(sRing >> 4);
     auto desc = [&](uint32_t address) { return like | (uint64_t)address; };
@@ -407,28 +405,29 @@ attention_packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
       return (like & ~((uint64_t)0x3fff << 16)) | ((uint64_t)(C::kBlock >> 4) << 16) | (uint64_t)address;
     };
     const int t = uniform(warp - kIssueWarp), q_tile = dual ? 0 : t;
-    const uint32_t d_s = tm + t * BN, a_p = C::kPlaceForP ? tm + C::kColP + t * 64 : d_s, d_o = tm + C::kColO + t * D;
+    const uint32_t d_s = tm + t * BN, d_o = tm + C::kColO + t * D;        // (P in the first half of its scores' place)
     int ring = 0, steps = 0, queries = 0;                      // ring tiles, steps, Q tiles of the pieces before
     for (int k = 0; wait(C::kTold + k % kPieces, k / kPieces); ++k) {
       const Piece& p = *piece_at(k);
       if (!p.more) break;
       const int n = uniform(p.n[t]), copied = uniform(p.copied), set = queries % C::kSets;
       const uint32_t dq = dq0 + uniform(2 * set + q_tile) * (C::kTile >> 4);
-      auto scores = [&](int i) {
+      // scores of half u of step i's keys; their place is free behind P V of the half that was there
+      auto scores = [&](int i, int u) {
         const int slot = ring + 2 * copy_of(t, i), st = uniform(slot % C::kStages);
         if (!wait(C::kFull + st, slot / C::kStages)) return;
-        if (steps + i > 0 && !wait((C::kPlaceForP ? C::kRead : C::kPv) + t, steps + i - 1)) return;       // the scores' place is free
+        if (steps + i > 0 && !wait(C::kPv + 2 * u + t, steps + i - 1)) return;
         fence_after_sync();
-        const uint32_t dk = dk0 + st * (C::kTile >> 4);
+        const uint32_t dk = dk0 + st * (C::kTile >> 4) + uniform(u) * (64 * 128 >> 4), to = d_s + uniform(u) * 64;
         if (elected) {
 #pragma unroll
           for (int k = 0; k < D / 16; ++k) {
             const uint32_t step = (k >> 2) * (C::kBlock >> 4) + 2 * (k & 3);
-            mma_bf16(d_s, desc(dq + step), desc(dk + step), kIdescS, k > 0);
+            mma_bf16(to, desc(dq + step), desc(dk + step), kIdescS, k > 0);
           }
-          mma_commit(bar(C::kS + t));
-          mma_commit(bar(C::kEmpty + st));
-          if (i + 1 == n) mma_commit(bar(C::kQUsed + 2 * set + q_tile));
+          mma_commit(bar(C::kS + 2 * u + t));
+          if (u) mma_commit(bar(C::kEmpty + st));
+          if (u && i + 1 == n) mma_commit(bar(C::kQUsed + 2 * set + q_tile));
         }
         __syncwarp();
       };
@@ -437,27 +436,27 @@ attention_packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
         ++queries;
         if (n == 0 && lane == 0) mbar_arrive(bar(C::kQUsed + 2 * set + q_tile));
       }
-      if (ok && n > 0) scores(0);
+      if (ok && n > 0) scores(0, 0);
+      if (ok && n > 0) scores(0, 1);
       for (int i = 0; i < n && ok; ++i) {
-        if (C::kPlaceForP && i + 1 < n) scores(i + 1);
         const int slot = ring + 2 * copy_of(t, i) + 1, st = uniform(slot % C::kStages);
-        if (!wait(C::kClean + st, slot / C::kStages) || !wait(C::kP + t, steps + i)) break;
+        if (!wait(C::kClean + st, slot / C::kStages)) break;
         const uint32_t dv = dk0 + st * (C::kTile >> 4), more = uniform(i > 0);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {                           // (the first half of the keys while the second half's weights are made)
-          if (h && !wait(C::kP + 2 + t, steps + i)) break;
+#pragma unroll 1
+        for (int u = 0; u < 2; ++u) {
+          if (!wait(C::kP + 2 * u + t, steps + i)) break;
           fence_after_sync();
+          const uint32_t from = dv + uniform(u) * (64 * 128 >> 4), a_p = d_s + uniform(u) * 64, first = uniform(u) | more;
           if (elected) {
 #pragma unroll
-            for (int k = 4 * h; k < 4 * h + 4; ++k) mma_bf16_a_tmem(d_o, a_p + k * 8, desc_v(dv + k * (2048 >> 4)), kIdescO, k > 0 ? 1u : more);
-            if (h) {
-              mma_commit(bar(C::kPv + t));
-              mma_commit(bar(C::kEmpty + st));
-            }
+            for (int k = 0; k < 4; ++k) mma_bf16_a_tmem(d_o, a_p + k * 8, desc_v(from + k * (2048 >> 4)), kIdescO, k > 0 ? 1u : first);
+            mma_commit(bar(C::kPv + 2 * u + t));
+            if (u) mma_commit(bar(C::kEmpty + st));
           }
           __syncwarp();
+          if (i + 1 < n) scores(i + 1, u);
+          if (!ok) break;
         }
-        if (!C::kPlaceForP && ok && i + 1 < n) scores(i + 1);
       }
       if (!dual)                          // tiles that only the other query tile uses: free for this one, each once it is there
         for (int c = 2 * n; c < 2 * copied && ok; ++c)
@@ -521,7 +520,7 @@ attention_packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
     // ---- the softmax groups ----
     const int t = warp >> 2, row = tid & (BM - 1);
     const uint32_t t_lane = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-    const uint32_t t_s = t_lane + t * BN, t_p = C::kPlaceForP ? t_lane + C::kColP + t * 64 : t_s, t_o = t_lane + C::kColO + t * D;
+    const uint32_t t_s = t_lane + t * BN, t_o = t_lane + C::kColO + t * D;
     const int local_token = row / G, local_head = row - local_token * G;      // of this thread's row in a query tile
     uint8_t* out_place = smem + C::kSmemTiles + warp * C::kOutBytes;
     const bool direct = a.n_rec <= 1;
@@ -542,93 +541,71 @@ attention_packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
       }
       const int lim_warp = __reduce_min_sync(0xffffffffu, lim);
       float m_ref = -INFINITY, l = 0.f;
-      for (int i = 0; i < n; ++i) {
-        const int key0 = (j0 + copy_of(t, i)) * BN, g = steps + i;
-        if (!wait(C::kS + t, g)) break;
+#pragma unroll 1
+      for (int half = 0; half < 2 * n; ++half) {                   // 64 keys at a time
+        const int i = half >> 1, u = half & 1, key0 = (j0 + copy_of(t, i)) * BN + 64 * u, g = steps + i;
+        if (!wait(C::kS + 2 * u + t, g)) break;
         fence_after_sync();
         if (busy) {
-          float s[BN];
-#pragma unroll
-          for (int c = 0; c < 4; ++c) tmem_ld32(t_s + 32 * c, s + 32 * c);
+          float x[64];
+          tmem_ld32(t_s + 64 * u, x);
+          tmem_ld32(t_s + 64 * u + 32, x + 32);
           tmem_ld_wait();
-          if (C::kPlaceForP) {
-            fence_before_sync();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar(C::kRead + t));
-          }
-          if (key0 + BN > lim_warp || key0 < lo) {
+          if (key0 + 64 > lim_warp || key0 < lo) {
             const int from = lo - key0, to = lim - key0;
 #pragma unroll
-            for (int c = 0; c < BN; ++c) s[c] = (c >= from && c < to) ? s[c] : -INFINITY;
+            for (int c = 0; c < 64; ++c) x[c] = (c >= from && c < to) ? x[c] : -INFINITY;
           }
-          float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          float top[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-          for (int c = 0; c < BN; c += 2) m4[(c >> 1) & 3] = max3_nan(m4[(c >> 1) & 3], s[c], s[c + 1]);
-          const float m_tile = max3_nan(max3_nan(m4[0], m4[1], m4[2]), m4[3], m4[3]) * a.scale_log2;
-          const bool move = !(m_tile <= m_ref + kMoveFrom);
+          for (int c = 4; c < 64; c += 2) top[(c >> 1) & 3] = max3_nan(top[(c >> 1) & 3], x[c], x[c + 1]);
+          const float m_new = max3_nan(max3_nan(top[0], top[1], top[2]), top[3], top[3]) * a.scale_log2;
+          const bool move = !(m_new <= m_ref + kMoveFrom);
           if (__any_sync(0xffffffffu, move)) {
-            // (0 on the first tile.  A row with a score that is no number, or infinite, becomes NaN as a whole.)
-            const float alpha = move ? fast_exp2(m_ref - m_tile) : 1.f;
-            if (move) m_ref = m_tile < INFINITY ? m_tile : NAN;
+            // (0 for the first keys.  A row with a score that is no number, or infinite, becomes NaN as a whole.)
+            const float alpha = move ? fast_exp2(m_ref - m_new) : 1.f;
+            if (move) m_ref = m_new < INFINITY ? m_new : NAN;
             l *= alpha;
-            if (i > 0) {
-              if (!wait(C::kPv + t, g - 1)) break;
+            if (half > 0) {
+              if (!wait(C::kPv + 2 * (u ^ 1) + t, u ? g : g - 1)) break;      // P V of the half before
               fence_after_sync();
 #pragma unroll 1
-              for (int c = 0; c < D; c += 32) {
-                float o[32];
-                tmem_ld32(t_o + c, o);
+              for (int c = 0; c < D; c += 16) {
+                float o[16];
+                tmem_ld16(t_o + c, o);
                 tmem_ld_wait();
 #pragma unroll
-                for (int e = 0; e < 32; ++e) o[e] *= alpha;
-                tmem_st32(t_o + c, o);
+                for (int e = 0; e < 16; ++e) o[e] *= alpha;
+                tmem_st16(t_o + c, reinterpret_cast<const uint32_t*>(o));
               }
               tmem_st_wait();
             }
           }
           const Two scale2(a.scale_log2), minus2(m_ref == -INFINITY ? 0.f : -m_ref);
           Two sum2[2] = {Two(0.f), Two(0.f)};
-          if (C::kPlaceForP && g > 0 && !wait(C::kPv + t, g - 1)) break;      // the tile before's P has been used
-          // The two warps of a scheduler that make exponentials do so one after the other where they can: the first is done in half the time,
-          // and its products run while the second is at it.  (No more than a hint: the wait ends by itself.)
-          if (!C::kPlaceForP) {
-            for (int polls = 0; s_turn[warp ^ 4] && polls < 64; ++polls) {}
-            s_turn[warp] = 1;
-          }
+          uint32_t packed[32];
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint32_t packed[BN / 4];
-#pragma unroll
-            for (int c = 0; c < BN / 4; ++c) {
-              float x, y;
-              fma2(Two(s[64 * h + 2 * c], s[64 * h + 2 * c + 1]), scale2, minus2).get(x, y);
-              x = fast_exp2(x);
-              y = fast_exp2(y);
-              sum2[c & 1] = sum2[c & 1] + Two(x, y);
-              const __nv_bfloat162 b = __floats2bfloat162_rn(x, y);
-              packed[c] = *reinterpret_cast<const uint32_t*>(&b);
-            }
-            tmem_st32(t_p + 32 * h, reinterpret_cast<const float*>(packed));
-            if (h == 1 && !C::kPlaceForP) s_turn[warp] = 0;
-            tmem_st_wait();
-            fence_before_sync();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar(C::kP + 2 * h + t));
+          for (int c = 0; c < 32; ++c) {
+            float p0, p1;
+            fma2(Two(x[2 * c], x[2 * c + 1]), scale2, minus2).get(p0, p1);
+            p0 = fast_exp2(p0);
+            p1 = fast_exp2(p1);
+            sum2[c & 1] = sum2[c & 1] + Two(p0, p1);
+            const __nv_bfloat162 b = __floats2bfloat162_rn(p0, p1);
+            packed[c] = *reinterpret_cast<const uint32_t*>(&b);
           }
-          float x, y;
-          (sum2[0] + sum2[1]).get(x, y);
-          l += x + y;
-        } else {
-          if (C::kPlaceForP) {
-            if (lane == 0) mbar_arrive(bar(C::kRead + t));
-            if (g > 0 && !wait(C::kPv + t, g - 1)) break;                     // (its arrivals below must not count for the step before)
-          }
-          __syncwarp();
-          if (lane == 0) { mbar_arrive(bar(C::kP + t)); mbar_arrive(bar(C::kP + 2 + t)); }
+          tmem_st32(t_s + 64 * u, reinterpret_cast<const float*>(packed));
+          float s0, s1;
+          (sum2[0] + sum2[1]).get(s0, s1);
+          l += s0 + s1;
+          tmem_st_wait();
         }
+        fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(C::kP + 2 * u + t));
       }
       steps += n;
-      if (n > 0) wait(C::kPv + t, steps - 1);
+      if (n > 0) wait(C::kPv + 2 + t, steps - 1);
       if (!ok) break;
       fence_after_sync();
       if (busy) {
