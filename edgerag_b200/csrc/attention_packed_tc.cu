@@ -619,18 +619,24 @@ attention_packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
         // Rows leave through shared memory, 64 bytes of each at a time: four lanes then write a row's piece side by side.
         const long long place = direct ? (long long)token * a.ld_out + (long long)head * D : (long long)record * D;
         const bool stored = mine && (direct || l != 0.f);
+        long long to[4];                                                      // the four rows that this lane writes a quarter of
+        unsigned store = 0;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          to[q] = __shfl_sync(0xffffffffu, place, 8 * q + (lane >> 2));
+          store |= (unsigned)__shfl_sync(0xffffffffu, (int)stored, 8 * q + (lane >> 2)) << q;
+        }
         auto leave = [&](const uint4* w, int col) {
 #pragma unroll
           for (int q = 0; q < 4; ++q) *reinterpret_cast<uint4*>(out_place + lane * 64 + ((q ^ ((lane >> 1) & 3)) << 4)) = w[q];
           __syncwarp();
 #pragma unroll
-          for (int r0 = 0; r0 < 32; r0 += 8) {
-            const int r = r0 + (lane >> 2), q = lane & 3;
-            const uint4 x = *reinterpret_cast<const uint4*>(out_place + r * 64 + ((q ^ ((r >> 1) & 3)) << 4));
-            const long long to = __shfl_sync(0xffffffffu, place, r);
-            if (!__shfl_sync(0xffffffffu, (int)stored, r)) continue;
-            if (direct) *reinterpret_cast<uint4*>(a.out + to + col + 8 * q) = x;
-            else *reinterpret_cast<uint4*>(a.part_o + to + col + 4 * q) = x;
+          for (int q = 0; q < 4; ++q) {
+            const int r = 8 * q + (lane >> 2), part = lane & 3;
+            const uint4 x = *reinterpret_cast<const uint4*>(out_place + r * 64 + ((part ^ ((r >> 1) & 3)) << 4));
+            if (!(store >> q & 1)) continue;
+            if (direct) *reinterpret_cast<uint4*>(a.out + to[q] + col + 8 * part) = x;
+            else *reinterpret_cast<uint4*>(a.part_o + to[q] + col + 4 * part) = x;
           }
           __syncwarp();
         };
