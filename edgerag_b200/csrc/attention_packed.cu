@@ -5,7 +5,8 @@
 // A block owns 32 rows of one kv head and walks its keys 64 at a time with the running maximum and sum of the softmax.  Queries, keys and
 // values lie in shared memory as floats; a thread of the 128 owns 4 x 4 scores and then 4 rows x D / 16 entries of the result, so that
 // 16 products take 8 floats from shared memory.  What bounds it: the fused multiply-adds of CUDA cores, and the
-// longest row tile's walk (5 prompts of up to 701 tokens, 15 heads of 64: tiles of 64 rows 113 us, of 32 84 us).
+// longest row tile's walk (5 prompts of up to 701 tokens, 15 heads of 64: tiles of 64 rows 113 us, of 32 84 us; with four steps of the scores'
+// loop unrolled, so that the next floats are asked for before these are used, 78 us; two multiply-adds an instruction: 80 us).
 //
 // Keys that no row of the block may see are zeros in shared memory, whatever their memory holds; where only some rows may see a key, its
 // product is left out for the others, not multiplied by zero, so that an infinity or NaN there stays unseen.
@@ -54,11 +55,15 @@ __global__ void __launch_bounds__(kThreads) attention_packed_kernel(const Packed
   extern __shared__ __align__(16) uint8_t raw[];
   Smem<DMAX>& sm = *reinterpret_cast<Smem<DMAX>*>(raw);
   constexpr int LD = Smem<DMAX>::kLd, LDP = Smem<DMAX>::kLdP, NC = DMAX / 64;
-  const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4, D = a.D, G = a.nq / a.nkv, kvh = blockIdx.y;
+  const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4, D = a.D, G = a.nq / a.nkv, kvh = MODE == kPrompt ? blockIdx.x % a.nkv : blockIdx.y;
 
   // the rows of this block: tokens t0 .. of one sequence (kPrefix: of all), rows r0 .. of them
   int seq = 0, tile = blockIdx.x, t0, len;
-  if (MODE == kPrompt) find_tile(a.seq_starts, a.n_seqs, G, BM, (int)(gridDim.x - 1 - blockIdx.x), seq, tile);
+  if (MODE == kPrompt) {           // the tiles that see the most keys first, each one's kv heads side by side
+    const TileList list(a.seq_starts, a.n_seqs, G, BM);
+    if ((int)(blockIdx.x / a.nkv) >= list.total) return;
+    list.find(blockIdx.x / a.nkv, seq, tile);
+  }
   if (MODE == kOwn) { seq = blockIdx.x / a.pieces; tile = 0; }
   if (seq < 0) return;
   if (MODE == kPrefix) {
@@ -185,6 +190,7 @@ __global__ void __launch_bounds__(kThreads) attention_packed_kernel(const Packed
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) s[i][j] = 0.f;
+#pragma unroll 4
       for (int c = 0; c < D; c += 4) {
         float4 qa[4], ka[4];
 #pragma unroll
@@ -338,8 +344,8 @@ ERB_EXPORT int erb_attention_prompt(const void* q, long long ld_q, const void* k
   a.seq_starts = seq_starts; a.n_seqs = n_seqs; a.n_tokens = n_tokens; a.nq = nq; a.nkv = nkv; a.D = head_dim;
   a.scale_log2 = scale * 1.4426950408889634f; a.n_rec = 1; a.pieces = 1; a.status = status; a.page_size = 1;
   const long long tiles = (long long)n_tokens * (nq / nkv) / BM + n_seqs;      // (a sequence has at most one tile that is not full)
-  if (tiles > 0x7fffffffLL) return fail(ERB_ERR_UNSUPPORTED, "attention_prompt: too many rows");
-  return launch_by_size<kPrompt>(a, dim3((unsigned)tiles, nkv, 1), (cudaStream_t)stream, "attention_prompt");
+  if (tiles * nkv > 0x7fffffffLL) return fail(ERB_ERR_UNSUPPORTED, "attention_prompt: too many rows");
+  return launch_by_size<kPrompt>(a, dim3((unsigned)(tiles * nkv), 1, 1), (cudaStream_t)stream, "attention_prompt");
 }
 
 // A batch that shares a prefix: keys 0 .. prefix_len - 1 of every sequence lie in the pages prefix_pages (int32), those from prefix_len on

@@ -128,59 +128,6 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
       ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
 }
 
-// The tiles of `rows` rows that the sequences give, those far along their sequences first (they see the most keys): how many there are, and
-// the sequence and tile of the index-th.  The whole warp asks; lane l keeps the tiles of sequences l, l + 32, .. apart.
-struct TileList {
-  const int* starts;
-  int n_seqs, G, rows, total, most;
-  int first_of_lane, start_of_lane, len_of_lane;              // of sequence `lane`
-  __device__ __forceinline__ int tiles(int s) const {
-    if (s >= n_seqs) return 0;
-    const long long pairs = (long long)max(0, __ldcg(starts + s + 1) - __ldcg(starts + s)) * G;
-    return (int)((pairs + rows - 1) / rows);
-  }
-  __device__ __forceinline__ int of(int s0) const { return s0 == 0 ? first_of_lane : tiles(s0 + (int)(threadIdx.x & 31)); }
-  __device__ __forceinline__ TileList(const int* starts, int n_seqs, int G, int rows) : starts(starts), n_seqs(n_seqs), G(G), rows(rows) {
-    start_of_lane = n_seqs > 0 ? __ldcg(starts + min((int)(threadIdx.x & 31), n_seqs - 1)) : 0;
-    len_of_lane = (int)(threadIdx.x & 31) < n_seqs ? __ldcg(starts + (threadIdx.x & 31) + 1) - start_of_lane : 0;
-    first_of_lane = (int)(((long long)max(0, len_of_lane) * G + rows - 1) / rows);
-    long long sum = 0;
-    most = 0;
-    for (int s0 = 0; s0 < n_seqs; s0 += 32) {
-      const int n = of(s0);
-      sum += __reduce_add_sync(0xffffffffu, n);
-      most = max(most, __reduce_max_sync(0xffffffffu, n));
-    }
-    total = (int)min(sum, (long long)0x3fffffff);
-  }
-  __device__ __forceinline__ int beyond(int level) const {      // tiles whose number in their sequence is at least `level`
-    int sum = 0;
-    for (int s0 = 0; s0 < n_seqs; s0 += 32) sum += __reduce_add_sync(0xffffffffu, max(0, of(s0) - level));
-    return sum;
-  }
-  __device__ __forceinline__ void find(int index, int& seq, int& tile) const {
-    int low = 0, high = most;                                   // beyond(low) > index >= beyond(high)
-    while (high - low > 1) {
-      const int mid = (low + high) >> 1;
-      if (beyond(mid) > index) low = mid;
-      else high = mid;
-    }
-    tile = low;
-    index -= beyond(low + 1);
-    seq = -1;
-    for (int s0 = 0; s0 < n_seqs; s0 += 32) {
-      const unsigned have = __ballot_sync(0xffffffffu, of(s0) > low);
-      const int count = __popc(have);
-      if (index < count) {
-        const int lane = threadIdx.x & 31;
-        seq = s0 + __ffs(__ballot_sync(0xffffffffu, (have >> lane & 1) && __popc(have & ((1u << lane) - 1)) == index)) - 1;
-        return;
-      }
-      index -= count;
-    }
-  }
-};
-
 template <int D, int MODE>
 __global__ void __launch_bounds__(kThreads, 1)
 attention_packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
