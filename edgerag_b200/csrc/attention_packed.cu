@@ -10,6 +10,7 @@
 //
 // Keys that no row of the block may see are zeros in shared memory, whatever their memory holds; where only some rows may see a key, its
 // product is left out for the others, not multiplied by zero, so that an infinity or NaN there stays unseen.
+#include <limits.h>
 #include <stdarg.h>
 
 #include "packed.cuh"
@@ -94,7 +95,7 @@ __global__ void __launch_bounds__(kThreads) attention_packed_kernel(const Packed
         const int token = (r0 + tid) / G;
         if (MODE == kPrompt) lim = token + 1;
         else {
-          lim = a.positions[t0 + token] + 1;
+          lim = max(0, min(a.positions[t0 + token], INT_MAX - 1) + 1);
           if (MODE == kPrefix) lim = min(lim, a.prefix_len);
           if (MODE == kOwn && lim > (long long)a.table_ld * a.page_size) { report(a.status, kBadPage); lim = a.table_ld * a.page_size; }
         }

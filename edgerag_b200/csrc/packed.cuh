@@ -161,9 +161,8 @@ __device__ __forceinline__ void join_records(const float* part_ml, const float* 
 #pragma unroll
   for (int h = 0; h < 4; ++h) {
     const int r = lane + 32 * h;
-    const float2 ml = r < n ? __ldcg(reinterpret_cast<const float2*>(part_ml) + r) : make_float2(-INFINITY, 0.f);
-    rm[h] = ml.x;
-    rl[h] = ml.y;
+    rm[h] = r < n ? __ldcg(part_ml + 2 * r) : -INFINITY;         // (the pair may lie on any float: one word at a time)
+    rl[h] = r < n ? __ldcg(part_ml + 2 * r + 1) : 0.f;
   }
   values(0);
 #pragma unroll

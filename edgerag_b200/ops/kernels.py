@@ -2345,7 +2345,7 @@ def rotary_append(q: torch.Tensor, positions: torch.Tensor, turns: torch.Tensor 
     Queries go to ``q_out`` (None: in place).  With ``k_pages`` and ``v_pages`` ``[pages, n_kv_heads, page_size, head_dim]``, keys and values (as
     they are) go to slot ``slots[token]`` (int32, ``page * page_size + offset``, no two alike; negative: nowhere), and keys to ``k_out`` only if it
     is given; without pages keys go to ``k_out`` (None: in place) and there is no ``v``.  A slot behind the pool is left alone and sets
-    ``status`` (int32) to the token's number plus one."""
+    ``status`` (int32) to the token's number plus one.  Beside the places named here, what is written overlaps no input."""
     who = "rotary_append"
     if q.dtype not in _ELEM or q.dim() != 2:
         raise KernelError(f"{who}: q must be rows of float32 or bfloat16")
@@ -2429,7 +2429,7 @@ def attention_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seq_star
     ``q`` and ``out`` ``[tokens, n_q_heads * head_dim]``, ``k`` and ``v`` ``[tokens, n_kv_heads * head_dim]`` (rows with any stride between them:
     views of one projection's rows); ``seq_starts`` int32 ``[n + 1]``, ascending: sequence ``s`` is rows ``seq_starts[s]`` to ``seq_starts[s + 1]``,
     possibly none.  Row ``i`` of a sequence sees its rows ``0 .. i``; query head ``h`` reads kv head ``h // (n_q_heads // n_kv_heads)``.  Rows outside
-    the sequences are left as they are.  Starts outside the rows set ``status`` (int32)."""
+    the sequences are left as they are; ``out`` overlaps no input.  Starts outside the rows set ``status`` (int32)."""
     who = "attention_prompt"
     if q.dtype not in _ELEM or q.dim() != 2:
         raise KernelError(f"{who}: q must be rows of float32 or bfloat16")
@@ -2446,7 +2446,8 @@ def attention_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seq_star
     _on_this_device(who, q, k, v, seq_starts, out, status)
     if n == 0 or seq_starts.numel() == 1:
         return
-    if packed_tc_supported(q.dtype, head_dim, n_q_heads // n_kv_heads) and _on_16_bytes(ld_q | ld_k | ld_v | ld_o, q, k, v, out) and min(ld_k, ld_v) >= n_kv_heads * head_dim:
+    if packed_tc_supported(q.dtype, head_dim, n_q_heads // n_kv_heads) and _on_16_bytes(ld_q | ld_k | ld_v | ld_o, q, k, v, out) and ld_q >= n_q_heads * head_dim \
+            and min(ld_k, ld_v) >= n_kv_heads * head_dim:
         fn = _fn("attention_packed_tc", None, "erb_attention_prompt_tc")
     else:
         fn = _fn("attention_packed", _elem(q), "erb_attention_prompt")
@@ -2497,6 +2498,8 @@ def shared_prefix_plan(n_tokens: int, n_seqs: int, n_q_heads: int, n_kv_heads: i
             each = 2 if prefix_dual else 1
             prefix_pieces = each * _cut(-(-prefix_len // (128 * each)), max(1, n_kv_heads * -(-n_tokens * group // (2 * tile))), sms, 3)
         own = OWN_TOKEN if max_tokens == 1 and group <= 16 else OWN_ROWS if max_tokens * group < 256 else OWN_MANY
+        if (n_seqs if own == OWN_TOKEN else n_tokens * group // 64 + n_seqs) > 65535:      # more blocks than their launches have places for
+            own = OWN_MANY
         if own == OWN_MANY:
             tiles = own_keys // 128 + 2 - (prefix_len % 128 == 0)
             cut = _cut(tiles, max(1, n_kv_heads * max(n_seqs, -(-n_tokens * group // (2 * tile)))), sms, 3)
@@ -2534,7 +2537,7 @@ def attention_shared_prefix(q: torch.Tensor, k_pages: torch.Tensor, v_pages: tor
     ``prefix_pages`` (int32): the pages of keys ``0 .. prefix_len - 1``; ``block_tables`` int32 ``[requests, entries]``: entry ``i`` is the page of
     a request's keys ``i * page_size ..`` (entries of pages wholly inside the prefix are not read; the page that the prefix ends in has a copy of
     the request's own).  ``plan`` is ``shared_prefix_plan``'s for these sizes, ``scratch`` float32 with ``plan.floats`` entries.  Rows outside the
-    requests are left as they are, a row that sees no key becomes zeros.  A page number outside the pool, a position behind the table or starts
+    requests are left as they are, a row that sees no key becomes zeros; ``out`` and ``scratch`` overlap no input.  A page number outside the pool, a position behind the table or starts
     outside the rows set ``status`` (int32); the results are then not valid."""
     who = "attention_shared_prefix"
     if q.dtype not in _ELEM or q.dim() != 2 or k_pages.dim() != 4:
@@ -2568,7 +2571,7 @@ def attention_shared_prefix(q: torch.Tensor, k_pages: torch.Tensor, v_pages: tor
         return
     part_o = scratch.data_ptr()
     if plan.tensor_cores and packed_tc_supported(q.dtype, head_dim, n_q_heads // n_kv_heads, page_size) and _on_16_bytes(ld_q | ld_o, q, out, k_pages, v_pages, scratch) \
-            and n_pages * n_kv_heads * page_size <= 0x7fffffff:
+            and ld_q >= n_q_heads * head_dim and n_pages * n_kv_heads * page_size <= 0x7fffffff:
         fn, how = _fn("attention_packed_tc", None, "erb_attention_shared_prefix_tc"), (int(plan.prefix_dual), plan.own)
     else:
         fn, how = _fn("attention_packed", _elem(q), "erb_attention_shared_prefix"), ()

@@ -440,3 +440,60 @@ def test_plans_cover_the_keys(rows, seqs, nq, nkv, dim, prefix, keys, fresh, dty
     assert p.own_pieces * p.piece_keys >= keys - prefix
     records = p.prefix_pieces + p.own_pieces
     assert p.floats >= (rows * nq * records * (dim + 2) if records > 1 else 0)
+
+
+def test_plans_of_very_many_requests_stay_launchable():
+    for rows, fresh in ((70000, 1), (70000, 2)):
+        p = K.shared_prefix_plan(rows, rows // fresh, 8, 8, 64, torch.bfloat16, 16, 64, 96, fresh, sms=148)
+        assert p.tensor_cores and (p.own == K.OWN_MANY or rows // fresh <= 65535 and p.own == K.OWN_ROWS and rows // 64 + rows // fresh <= 65535)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("elem", ["float32", "bfloat16"])
+@pytest.mark.parametrize("shift", [0, 1, 2])
+@pytest.mark.parametrize("dim", [5, 15, 64])
+def test_records_at_any_place_of_the_scratch(elem, shift, dim):
+    """An odd number of odd records, or a scratch that is a part of a larger buffer: maxima and sums then lie on no 8-byte boundary."""
+    c = shared_call(elem, 200, (1,), (70,), 1, 1, dim, 16)
+    plan = K.SharedPrefixPlan(2, 1, 4096, 3 * (dim + 2))
+    n, width = c["q"].shape[0], c["nq"] * dim
+    out, status = torch.zeros((n, width), dtype=c["q"].dtype).cuda(), torch.zeros(1, dtype=torch.int32).cuda()
+    scratch = torch.full((shift + plan.floats,), float("nan")).cuda()[shift:]
+    K.attention_shared_prefix(c["q"].cuda(), c["k"].cuda(), c["v"].cuda(), c["prefix_pages"].cuda(), c["prefix"], c["tables"].cuda(), c["starts"].cuda(),
+                              c["positions"].cuda(), out, c["nq"], c["scale"], plan, scratch, status)
+    assert int(status) == 0
+    check_shared(c, out.cpu())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("elem,dim", [("bfloat16", 64), ("bfloat16", 128), ("float32", 64), ("bfloat16", 40)])
+@pytest.mark.parametrize("fresh", [(1, 1), (1, 3), (150, 130)])
+def test_the_last_position_of_all_is_reported(elem, dim, fresh):
+    """Position 2^31 - 1, whose number of keys an int cannot hold, is behind every table."""
+    c = shared_call(elem, 100, fresh, (20, 30), 4, 2, dim, 16)
+    c["positions"][-1] = 2**31 - 1
+    _, status = run_shared(c)
+    assert status == 9000001
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("elem", ["float32", "bfloat16"])
+def test_one_row_of_queries_for_all(elem):
+    """Queries whose rows have no stride between them (one row, expanded)."""
+    rows, starts, scale = prompt_call(elem, (40, 130), 4, 2, 64)
+    one = rows[:1, :256].clone().cuda()
+    dev = rows.cuda()
+    out, status = torch.zeros((170, 256), dtype=rows.dtype).cuda(), torch.zeros(1, dtype=torch.int32).cuda()
+    K.attention_prompt(one.expand(170, 256), dev[:, 256:384], dev[:, 384:512], starts.cuda(), out, 4, 2, scale, status)
+    rows[:, :256] = one.cpu()
+    assert int(status) == 0
+    check_prompt(rows, starts, 4, 2, 64, scale, out.cpu())
+    c = shared_call(elem, 200, (1, 2), (10, 150), 4, 2, 64, 16)
+    want, _ = run_shared({**c, "q": c["q"][:1].repeat(3, 1)})
+    plan = K.shared_prefix_plan(3, 2, 4, 2, 64, c["q"].dtype, 16, 200, c["max_keys"], 2, sms=c["sms"])
+    got, scratch = torch.zeros((3, 256), dtype=rows.dtype).cuda(), torch.zeros(max(plan.floats, 1)).cuda()
+    K.attention_shared_prefix(c["q"][:1].cuda().expand(3, 256), c["k"].cuda(), c["v"].cuda(), c["prefix_pages"].cuda(), 200, c["tables"].cuda(), c["starts"].cuda(),
+                              c["positions"].cuda(), got, 4, c["scale"], plan, scratch, status)
+    c["q"] = c["q"][:1].repeat(3, 1)
+    assert int(status) == 0 and torch.isfinite(want).all()
+    check_shared(c, got.cpu())
