@@ -3,8 +3,8 @@
 //
 // A piece of work is up to 256 rows of one kv head, (token, head of its group) pairs, as two query tiles A and B of up to 128 rows, and a
 // walk over its keys in tiles of 128.  Every byte of K and V that reaches shared memory serves all its rows; with G query heads a kv head
-// a prompt's piece spans 256 / G tokens, so little of the last tile on the diagonal is hidden.  A call whose rows all fit one tile (`dual`)
-// gives both tiles the same rows and every other key tile each, and leaves a record of its sums for each of them.
+// a prompt's piece spans 256 / G tokens, so little of the last tile on the diagonal is hidden.  (Rows that all fit one tile leave the other idle:
+// with the same rows in both and every other key tile each, the ring is too short for two walks, and 128 rows over 16,384 keys took 40 us, not 32.)
 //
 // One block a multiprocessor takes pieces in turn, longest first (forwards and backwards through the list, so that the blocks' sums are
 // alike).  Its warps work by role, each as far ahead as the barriers let it, so that a piece's first copies and products run while the
@@ -131,7 +131,7 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
 template <int D, int MODE>
 __global__ void __launch_bounds__(kThreads, 1)
 attention_packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-                           const PackedArgs a, const int dual) {
+                           const PackedArgs a) {
   using C = Cfg<D>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
@@ -143,13 +143,13 @@ attention_packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
   auto bar = [&](int which) { return bars + 8u * (uint32_t)which; };
   auto piece_at = [&](int k) { return reinterpret_cast<Piece*>(smem + C::kSmemOut + 8 * C::kNumBars + 16 + (k % kPieces) * 64); };
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int G = a.nq / a.nkv, RT = BM / G * G, per_piece = dual ? RT : 2 * RT;      // rows of a query tile (whole tokens), of a piece
+  const int G = a.nq / a.nkv, RT = BM / G * G, per_piece = 2 * RT;      // rows of a query tile (whole tokens), of a piece
 
   if (tid == 0) {
-    for (int s = 0; s < C::kStages; ++s) { mbar_init(bar(C::kFull + s), 1); mbar_init(bar(C::kEmpty + s), dual ? 1 : 2); mbar_init(bar(C::kClean + s), 1); }
+    for (int s = 0; s < C::kStages; ++s) { mbar_init(bar(C::kFull + s), 1); mbar_init(bar(C::kEmpty + s), 2); mbar_init(bar(C::kClean + s), 1); }
     for (int k = 0; k < kPieces; ++k) { mbar_init(bar(C::kTold + k), 1); mbar_init(bar(C::kTaken + k), kSoftmaxWarps + 3); }
     for (int t = 0; t < 2; ++t) {
-      for (int s = 0; s < C::kSets; ++s) { mbar_init(bar(C::kQ + 2 * s + t), 1); mbar_init(bar(C::kQUsed + 2 * s + t), dual ? 2 : 1); }
+      for (int s = 0; s < C::kSets; ++s) { mbar_init(bar(C::kQ + 2 * s + t), 1); mbar_init(bar(C::kQUsed + 2 * s + t), 1); }
       for (int u = 0; u < 2; ++u) {
         mbar_init(bar(C::kS + 2 * u + t), 1);
         mbar_init(bar(C::kP + 2 * u + t), 4);
@@ -174,7 +174,6 @@ attention_packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
     if (ok && !__all_sync(0xffffffffu, mbar_try_some(bar(which), phase & 1))) ok = wait_long(bar(which), phase & 1, s_abort);
     return ok;
   };
-  auto copy_of = [&](int t, int i) { return dual ? 2 * i + t : i; };
   auto on_edge = [&](const Piece& p, int c) {          // some row sees only some of the tile's keys
     const int key0 = (p.j0 + c) * BN;
     return key0 < p.lo || key0 + BN > min(p.least[0], p.least[1]);
@@ -241,13 +240,13 @@ attention_packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
         }
         const int r0 = tile * per_piece, token_tile = RT / G;                  // (tokens times G is below 2^30)
         p.rows = min(per_piece, len * G - r0);
-        p.token0 = p.t0 + tile * (dual ? token_tile : 2 * token_tile);
+        p.token0 = p.t0 + tile * 2 * token_tile;
         // the keys that the rows of each query tile see
         int most[2] = {0, 0};
         p.least[0] = p.least[1] = INT_MAX;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          const int before = dual ? 0 : t * token_tile, n_tokens = max(0, min(token_tile, min((dual ? 1 : 2) * token_tile, p.t0 + len - p.token0) - before));
+          const int before = t * token_tile, n_tokens = max(0, min(token_tile, p.t0 + len - p.token0 - before));
           if (MODE == kPrompt) {
             if (n_tokens > 0) {
               p.least[t] = p.token0 - p.t0 + before + 1;
@@ -278,8 +277,8 @@ attention_packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
         }
         p.copied = j1 - p.j0;
 #pragma unroll
-        for (int t = 0; t < 2; ++t) p.n[t] = dual ? (p.copied - t + 1) / 2 : max(0, min(p.copied, (most[t] + BN - 1) / BN - p.j0));
-        if (!dual) p.copied = max(p.n[0], p.n[1]);
+        for (int t = 0; t < 2; ++t) p.n[t] = max(0, min(p.copied, (most[t] + BN - 1) / BN - p.j0));
+        p.copied = max(p.n[0], p.n[1]);
       }
       if (n_told >= kPieces && !wait(C::kTaken + n_told % kPieces, n_told / kPieces - 1)) break;
       if (lane == 0) {
@@ -289,7 +288,7 @@ attention_packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
       ++n_told;
       if (!p.more) break;
       // queries: whole tokens, the heads of the group in order (tokens behind the sequence's last one are rows that nobody stores)
-      for (int t = 0; t < (dual ? 1 : 2); ++t) {
+      for (int t = 0; t < 2; ++t) {
         if (p.n[t] == 0) continue;
         const int set = copies_q[t] % C::kSets, use = copies_q[t] / C::kSets;
         if (use > 0 && !wait(C::kQUsed + 2 * set + t, use - 1)) break;
@@ -351,17 +350,17 @@ attention_packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
     auto desc_v = [&](uint32_t address) {                      // 64 columns of V apart: a block
       return (like & ~((uint64_t)0x3fff << 16)) | ((uint64_t)(C::kBlock >> 4) << 16) | (uint64_t)address;
     };
-    const int t = uniform(warp - kIssueWarp), q_tile = dual ? 0 : t;
+    const int t = uniform(warp - kIssueWarp);
     const uint32_t d_s = tm + t * BN, d_o = tm + C::kColO + t * D;        // (P in the first half of its scores' place)
     int ring = 0, steps = 0, queries = 0;                      // ring tiles, steps, Q tiles of the pieces before
     for (int k = 0; wait(C::kTold + k % kPieces, k / kPieces); ++k) {
       const Piece& p = *piece_at(k);
       if (!p.more) break;
       const int n = uniform(p.n[t]), copied = uniform(p.copied), set = queries % C::kSets;
-      const uint32_t dq = dq0 + uniform(2 * set + q_tile) * (C::kTile >> 4);
+      const uint32_t dq = dq0 + uniform(2 * set + t) * (C::kTile >> 4);
       // scores of half u of step i's keys; their place is free behind P V of the half that was there
       auto scores = [&](int i, int u) {
-        const int slot = ring + 2 * copy_of(t, i), st = uniform(slot % C::kStages);
+        const int slot = ring + 2 * i, st = uniform(slot % C::kStages);
         if (!wait(C::kFull + st, slot / C::kStages)) return;
         if (steps + i > 0 && !wait(C::kPv + 2 * u + t, steps + i - 1)) return;
         fence_after_sync();
@@ -374,19 +373,18 @@ attention_packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
           }
           mma_commit(bar(C::kS + 2 * u + t));
           if (u) mma_commit(bar(C::kEmpty + st));
-          if (u && i + 1 == n) mma_commit(bar(C::kQUsed + 2 * set + q_tile));
+          if (u && i + 1 == n) mma_commit(bar(C::kQUsed + 2 * set + t));
         }
         __syncwarp();
       };
-      if (p.n[q_tile] > 0) {
-        wait(C::kQ + 2 * set + q_tile, queries / C::kSets);
+      if (n > 0) {
+        wait(C::kQ + 2 * set + t, queries / C::kSets);
         ++queries;
-        if (n == 0 && lane == 0) mbar_arrive(bar(C::kQUsed + 2 * set + q_tile));
       }
       if (ok && n > 0) scores(0, 0);
       if (ok && n > 0) scores(0, 1);
       for (int i = 0; i < n && ok; ++i) {
-        const int slot = ring + 2 * copy_of(t, i) + 1, st = uniform(slot % C::kStages);
+        const int slot = ring + 2 * i + 1, st = uniform(slot % C::kStages);
         if (!wait(C::kClean + st, slot / C::kStages)) break;
         const uint32_t dv = dk0 + st * (C::kTile >> 4), more = uniform(i > 0);
 #pragma unroll 1
@@ -405,9 +403,9 @@ attention_packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
           if (!ok) break;
         }
       }
-      if (!dual)                          // tiles that only the other query tile uses: free for this one, each once it is there
-        for (int c = 2 * n; c < 2 * copied && ok; ++c)
-          if (wait(C::kFull + (ring + c) % C::kStages, (ring + c) / C::kStages) && lane == 0) mbar_arrive(bar(C::kEmpty + (ring + c) % C::kStages));
+      // tiles that only the other query tile uses: free for this one, each once it is there
+      for (int c = 2 * n; c < 2 * copied && ok; ++c)
+        if (wait(C::kFull + (ring + c) % C::kStages, (ring + c) / C::kStages) && lane == 0) mbar_arrive(bar(C::kEmpty + (ring + c) % C::kStages));
       steps += n;
       ring += 2 * copied;
       taken(k);
@@ -475,9 +473,9 @@ attention_packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
     for (int k = 0; wait(C::kTold + k % kPieces, k / kPieces); ++k) {
       const Piece& p = *piece_at(k);
       if (!p.more) break;
-      const int index = (dual ? 0 : t * RT) + row, rows = p.rows, n = p.n[t], lo = p.lo, j0 = p.j0;
+      const int index = t * RT + row, rows = p.rows, n = p.n[t], lo = p.lo, j0 = p.j0;
       const bool mine = row < RT && index < rows, busy = __any_sync(0xffffffffu, mine);    // (rows do not meet: P of the others may be anything)
-      const int token = p.token0 + (dual ? 0 : t * (RT / G)) + local_token, head = p.kvh * G + local_head;
+      const int token = p.token0 + t * (RT / G) + local_token, head = p.kvh * G + local_head;
       int lim = INT_MAX;                                             // (a row that is none costs no mask)
       if (mine) {
         if (MODE == kPrompt) lim = token - p.t0 + 1;
@@ -490,7 +488,7 @@ attention_packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
       float m_ref = -INFINITY, l = 0.f;
 #pragma unroll 1
       for (int half = 0; half < 2 * n; ++half) {                   // 64 keys at a time
-        const int i = half >> 1, u = half & 1, key0 = (j0 + copy_of(t, i)) * BN + 64 * u, g = steps + i;
+        const int i = half >> 1, u = half & 1, key0 = (j0 + i) * BN + 64 * u, g = steps + i;
         if (!wait(C::kS + 2 * u + t, g)) break;
         fence_after_sync();
         if (busy) {
@@ -558,7 +556,7 @@ attention_packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
       if (busy) {
         const bool fix = *reinterpret_cast<const volatile int*>(&p.bad) != 0;
         const float inv = l != 0.f ? 1.f / l : 0.f;                           // (a row that sees no key: zeros)
-        const size_t record = ((size_t)token * a.nq + head) * a.n_rec + a.rec0 + (dual ? 2 * p.part + t : p.part);
+        const size_t record = ((size_t)token * a.nq + head) * a.n_rec + a.rec0 + p.part;
         if (!direct && mine) {
           a.part_ml[2 * record] = m_ref;
           a.part_ml[2 * record + 1] = l;
@@ -601,8 +599,8 @@ attention_packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
             // what this row does see of the values that were taken out
             const int* table = MODE == kOwn ? a.tables + (size_t)p.seq * a.table_ld : a.prefix_pages;
             for (int i = 0; i < n; ++i) {
-              if (!on_edge(p, copy_of(t, i))) continue;
-              const int key0 = (j0 + copy_of(t, i)) * BN;
+              if (!on_edge(p, i)) continue;
+              const int key0 = (j0 + i) * BN;
               for (int key = max(key0, lo); key < min(key0 + BN, lim); ++key) {
                 const elem_t *kr, *vr;
                 key_rows<MODE>(a, table, p.t0, p.kvh, key, kr, vr);
@@ -667,7 +665,7 @@ int query_map(CUtensorMap* out, const PackedArgs& a, const char* who) {
 }
 
 template <int D, int MODE>
-int launch_one(const PackedArgs& a, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, long long pieces, int dual, cudaStream_t stream,
+int launch_one(const PackedArgs& a, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, long long pieces, cudaStream_t stream,
                const char* who) {
   static bool configured[64] = {};
   int dev = 0;
@@ -682,22 +680,22 @@ int launch_one(const PackedArgs& a, const CUtensorMap& mq, const CUtensorMap& mk
   }
   if (pieces > 0x7f000000LL) return fail(ERB_ERR_UNSUPPORTED, "%s: too many rows", who);
   launch_chained(attention_packed_tc_kernel<D, MODE>, dim3((unsigned)(pieces < sm_count() ? pieces : sm_count())), dim3(kThreads), Cfg<D>::kSmemBytes, stream,
-                 mq, mk, mv, a, dual);
+                 mq, mk, mv, a);
   return check_launch(who);
 }
 
 // pieces: a bound on the pieces of work.
 template <int MODE>
-int launch_tc(const PackedArgs& a, const CUtensorMap& mk, const CUtensorMap& mv, long long pieces, int dual, cudaStream_t stream, const char* who) {
+int launch_tc(const PackedArgs& a, const CUtensorMap& mk, const CUtensorMap& mv, long long pieces, cudaStream_t stream, const char* who) {
   CUtensorMap mq;
   if (const int rc = query_map(&mq, a, who)) return rc;
-  return a.D == 64 ? launch_one<64, MODE>(a, mq, mk, mv, pieces, dual, stream, who) : launch_one<128, MODE>(a, mq, mk, mv, pieces, dual, stream, who);
+  return a.D == 64 ? launch_one<64, MODE>(a, mq, mk, mv, pieces, stream, who) : launch_one<128, MODE>(a, mq, mk, mv, pieces, stream, who);
 }
 
-// Rows of a piece of work: whole tokens of G heads in one query tile or two.
-long long rows_of_piece(int G, int dual) { return (long long)(BM / G * G) * (dual ? 1 : 2); }
+// Rows of a piece of work: whole tokens of G heads in two query tiles.
+long long rows_of_piece(int G) { return 2LL * (BM / G * G); }
 
-// A request's own keys by the kernels for few rows: rows 1: one token a request (or one after the other), up to 16 query heads a kv head.
+// A request's own keys by the kernels for few rows: the one for a token a request (or one after the other) or the one for 64 rows.
 template <int D>
 int launch_few(const PackedArgs& a, bool one_token, int early, cudaStream_t stream, const char* who) {
   auto kern = one_token ? attention_own_token_kernel<D> : attention_own_rows_kernel<D>;
@@ -738,23 +736,22 @@ ERB_EXPORT int erb_attention_prompt_tc(const void* q, long long ld_q, const void
   if ((rc = rows_map(&mk, k, n_tokens, nkv * head_dim, ld_k, BN, "attention_prompt_tc")) ||
       (rc = rows_map(&mv, v, n_tokens, nkv * head_dim, ld_v, BN, "attention_prompt_tc")))
     return rc;
-  const long long pieces = ((long long)n_tokens * (nq / nkv) / rows_of_piece(nq / nkv, 0) + n_seqs) * nkv;      // (a sequence has at most one that is not full)
-  return launch_tc<kPrompt>(a, mk, mv, pieces, 0, (cudaStream_t)stream, "attention_prompt_tc");
+  const long long pieces = ((long long)n_tokens * (nq / nkv) / rows_of_piece(nq / nkv) + n_seqs) * nkv;      // (a sequence has at most one that is not full)
+  return launch_tc<kPrompt>(a, mk, mv, pieces, (cudaStream_t)stream, "attention_prompt_tc");
 }
 
 // The arguments of erb_attention_shared_prefix (attention_packed.cu); heads of 64 or 128, rows, their strides and the pools on 16-byte
-// boundaries, pages of 8 to 128 tokens, a power of two.  prefix_dual: blocks own 128 rows and leave two records each, so that prefix_pieces
-// is twice the blocks' pieces.  own: the kernel for a request's own keys (kOwnMany: this file's for many rows; kOwnToken, kOwnRows:
+// boundaries, pages of 8 to 128 tokens, a power of two.  own: the kernel for a request's own keys (kOwnMany: this file's for many rows; kOwnToken, kOwnRows:
 // packed_few.cuh's, which join the records themselves where own_pieces is 1).
 ERB_EXPORT int erb_attention_shared_prefix_tc(const void* q, long long ld_q, const void* k_pages, const void* v_pages, int n_pages, int page_size,
                                               const int* prefix_pages, int prefix_len, const int* tables, int table_ld, const int* seq_starts,
                                               const int* positions, int n_seqs, int n_tokens, void* out, long long ld_out, int nq, int nkv,
-                                              int head_dim, float scale, int prefix_pieces, int own_pieces, int piece_keys, int prefix_dual,
-                                              int own, float* part_o, float* part_ml, int* status, void* stream) {
+                                              int head_dim, float scale, int prefix_pieces, int own_pieces, int piece_keys, int own,
+                                              float* part_o, float* part_ml, int* status, void* stream) {
   if (n_seqs <= 0 || n_tokens <= 0) return ERB_OK;
   if (nq <= 0 || nkv <= 0 || nq % nkv || !status || n_pages <= 0 || prefix_len < 0 || table_ld <= 0 || prefix_pieces < (prefix_len > 0 ? 1 : 0) ||
       own_pieces < 1 || piece_keys <= 0 || !(scale > 0.f) || prefix_pieces > 64 ||
-      (prefix_dual && prefix_pieces % 2) || own < kOwnMany || own > kOwnRows || (own == kOwnToken && nq / nkv > 16))
+      own < kOwnMany || own > kOwnRows || (own == kOwnToken && nq / nkv > 16))
     return fail(ERB_ERR_ARG, "attention_shared_prefix_tc: bad sizes");
   if ((head_dim != 64 && head_dim != 128) || nq / nkv > BM || !aligned(q, ld_q) || !aligned(out, ld_out) || !aligned(k_pages, 0) || !aligned(v_pages, 0) ||
       page_size < 8 || page_size > BN || (page_size & (page_size - 1)) || (unsigned long long)n_pages * nkv * page_size > 0x7fffffffull)
@@ -777,13 +774,13 @@ ERB_EXPORT int erb_attention_shared_prefix_tc(const void* q, long long ld_q, con
   const long long rows = (long long)n_tokens * (nq / nkv);
   if (prefix_len > 0) {
     a.rec0 = 0;
-    a.pieces = prefix_dual ? prefix_pieces / 2 : prefix_pieces;
-    if ((rc = launch_tc<kPrefix>(a, mk, mv, (rows / rows_of_piece(nq / nkv, prefix_dual) + 1) * nkv * a.pieces, prefix_dual, s, who))) return rc;
+    a.pieces = prefix_pieces;
+    if ((rc = launch_tc<kPrefix>(a, mk, mv, (rows / rows_of_piece(nq / nkv) + 1) * nkv * a.pieces, s, who))) return rc;
   }
   a.rec0 = prefix_len > 0 ? prefix_pieces : 0;
   a.pieces = own_pieces;
   if (own == kOwnMany) {
-    if ((rc = launch_tc<kOwn>(a, mk, mv, (rows / rows_of_piece(nq / nkv, 0) + n_seqs) * nkv * a.pieces, 0, s, who)) || n_rec <= 1) return rc;
+    if ((rc = launch_tc<kOwn>(a, mk, mv, (rows / rows_of_piece(nq / nkv) + n_seqs) * nkv * a.pieces, s, who)) || n_rec <= 1) return rc;
   } else {
     rc = head_dim == 64 ? launch_few<64>(a, own == kOwnToken, prefix_len > 0, s, who) : launch_few<128>(a, own == kOwnToken, prefix_len > 0, s, who);
     if (rc || own_pieces == 1) return rc;

@@ -155,7 +155,7 @@ _SIGNATURES = {
                                 c_int, c_int, c_int, c_float, c_void_p, c_void_p],
     "erb_attention_shared_prefix_tc": [c_void_p, c_longlong, c_void_p, c_void_p, c_int, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p,
                                        c_void_p, c_int, c_int, c_void_p, c_longlong, c_int, c_int, c_int, c_float, c_int, c_int, c_int,
-                                       c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p],
+                                       c_int, c_void_p, c_void_p, c_void_p, c_void_p],
     "erb_attention_shared_prefix": [c_void_p, c_longlong, c_void_p, c_void_p, c_int, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p,
                                     c_void_p, c_int, c_int, c_void_p, c_longlong, c_int, c_int, c_int, c_float, c_int, c_int, c_int,
                                     c_void_p, c_void_p, c_void_p, c_void_p],
@@ -2463,8 +2463,7 @@ class SharedPrefixPlan(NamedTuple):
     piece_keys: int
     floats: int              # float32 entries of scratch
     tensor_cores: bool = False
-    prefix_dual: bool = False      # tensor cores: a block's two query tiles are the same 128 rows, each with half of the keys and a record of its own
-    own: int = 0                   # tensor cores: who takes a request's own keys (OWN_MANY, OWN_TOKEN, OWN_ROWS)
+    own: int = 0             # tensor cores: who takes a request's own keys (OWN_MANY, OWN_TOKEN, OWN_ROWS)
 
 
 OWN_MANY, OWN_TOKEN, OWN_ROWS = 0, 1, 2
@@ -2481,6 +2480,18 @@ def _cut(tiles: int, blocks: int, sms: int, fixed: int) -> int:
     return best[1]
 
 
+def _cut_prefix(tiles: int, blocks: int, own_blocks: int, sms: int) -> int:
+    """``_cut`` for a prefix whose requests' own keys are small blocks that run beside it (``own_blocks``, four a multiprocessor): where they
+    do not fit onto the multiprocessors that it leaves, it leaves a sixth of them, if that makes it less than a quarter longer.  64 requests,
+    16,384 keys, 8 kv heads of 128, 500 own keys each: 16 pieces 69 us, 15 62; 16 requests, 2,048 keys: 16 pieces 17.5 us, 8 13.8.  Where a
+    sixth costs more it does not pay: 64 requests, 32 kv heads of 64, 4,096 keys: 4 pieces 35 us, 3 38."""
+    full, most = _cut(tiles, blocks, sms, 4), sms - sms // 6
+    fewer = _cut(tiles, blocks, most, 4)
+    if full * blocks > sms or own_blocks <= 4 * (sms - full * blocks) or fewer * blocks > most:
+        return full
+    return fewer if 4 * (-(-tiles // fewer) + 4) < 5 * (-(-tiles // full) + 4) else full
+
+
 def shared_prefix_plan(n_tokens: int, n_seqs: int, n_q_heads: int, n_kv_heads: int, head_dim: int, dtype: torch.dtype, page_size: int,
                        prefix_len: int, max_keys: int, max_tokens: int = 1, sms: int | None = None) -> SharedPrefixPlan:
     """The plan for a batch of ``n_tokens`` rows of ``n_seqs`` requests: ``max_keys`` bounds the longest context, ``max_tokens`` a request's rows in
@@ -2491,27 +2502,32 @@ def shared_prefix_plan(n_tokens: int, n_seqs: int, n_q_heads: int, n_kv_heads: i
     sms = _sms(torch.device("cuda", torch._C._cuda_getDevice())) if sms is None else sms
     own_keys = max(1, max_keys - prefix_len)
     if packed_tc_supported(dtype, head_dim, n_q_heads // n_kv_heads, page_size):
-        group, prefix_pieces = n_q_heads // n_kv_heads, 0
+        group = n_q_heads // n_kv_heads
         tile = 128 // group * group            # rows of a query tile: whole tokens
-        prefix_dual = n_tokens * group <= tile
-        if prefix_len:
-            each = 2 if prefix_dual else 1
-            prefix_pieces = each * _cut(-(-prefix_len // (128 * each)), max(1, n_kv_heads * -(-n_tokens * group // (2 * tile))), sms, 3)
-        own = OWN_TOKEN if max_tokens == 1 and group <= 16 else OWN_ROWS if max_tokens * group < 256 else OWN_MANY
+        # One token a request: 500 own keys of 64 requests behind 16,384, 8 kv heads of 128, 69 us by the kernel for one token, 112 by the one for
+        # 64 rows, 102 by the one for many; 4,000 own keys of 4: 34, 57, 49.  Several: the one for 64 rows saves the many-row kernel's fixed time
+        # (24 requests, 16 kv heads of 64, 32 rows of 96 keys: 44 | 50 us, 100 rows 102 | 101; 4 requests 34 | 29) but is slower over long
+        # keys and larger heads (8 of 128, 24 requests, 32 rows of 72 keys 44 | 42, of 708 92 | 69; 8 rows of 66 keys 35 | 39).
+        rows = max_tokens * group
+        own = OWN_TOKEN if max_tokens == 1 and group <= 16 else OWN_MANY
+        if own == OWN_MANY and (rows <= 16 and own_keys <= 128 or head_dim == 64 and n_kv_heads * n_seqs > sms and rows <= 64 and own_keys <= 1024):
+            own = OWN_ROWS
         if (n_seqs if own == OWN_TOKEN else n_tokens * group // 64 + n_seqs) > 65535:      # more blocks than their launches have places for
             own = OWN_MANY
+        prefix_blocks = max(1, n_kv_heads * -(-n_tokens * group // (2 * tile)))
         if own == OWN_MANY:
             tiles = own_keys // 128 + 2 - (prefix_len % 128 == 0)
             cut = _cut(tiles, max(1, n_kv_heads * max(n_seqs, -(-n_tokens * group // (2 * tile)))), sms, 3)
             piece_keys = -(-tiles // cut) * 128
+            prefix_pieces = _cut(-(-prefix_len // 128), prefix_blocks, sms, 4) if prefix_len else 0
         else:       # small blocks, four a multiprocessor; with one piece there is no separate merge
             blocks = n_kv_heads * max(1, n_seqs if own == OWN_TOKEN else -(-n_tokens * group // 64))
             cut = min(max(1, 4 * sms // blocks), max(1, own_keys // 512), 64)
             piece_keys = -(-own_keys // (64 * cut)) * 64
+            prefix_pieces = _cut_prefix(-(-prefix_len // 128), prefix_blocks, blocks * cut, sms) if prefix_len else 0
         own_pieces = max(1, -(-(tiles * 128 if own == OWN_MANY else own_keys) // piece_keys))
         records = prefix_pieces + own_pieces
-        return SharedPrefixPlan(prefix_pieces, own_pieces, piece_keys, n_tokens * n_q_heads * records * (head_dim + 2) if records > 1 else 0, True,
-                                prefix_dual, own)
+        return SharedPrefixPlan(prefix_pieces, own_pieces, piece_keys, n_tokens * n_q_heads * records * (head_dim + 2) if records > 1 else 0, True, own)
     # Two blocks a multiprocessor, tiles of 64 keys, two tiles a piece at least.
     rows = n_tokens * (n_q_heads // n_kv_heads)
     blocks = max(1, -(-rows // 32) * n_kv_heads)
@@ -2562,7 +2578,7 @@ def attention_shared_prefix(q: torch.Tensor, k_pages: torch.Tensor, v_pages: tor
     if n * (n_q_heads // n_kv_heads) >= 1 << 30 or n_seqs >= 1 << 24:
         raise KernelError(f"{who}: {n} tokens of {n_q_heads} heads in one call")
     records = plan.prefix_pieces + plan.own_pieces
-    if (plan.prefix_dual and plan.prefix_pieces % 2) or (plan.own == OWN_TOKEN and n_q_heads // n_kv_heads > 16) or plan.own not in (OWN_MANY, OWN_TOKEN, OWN_ROWS) or plan.own_pieces < 1 or plan.own_pieces > 64 or plan.piece_keys < 1 or not (1 if prefix_len else 0) <= plan.prefix_pieces <= (64 if prefix_len else 0):
+    if (plan.own == OWN_TOKEN and n_q_heads // n_kv_heads > 16) or plan.own not in (OWN_MANY, OWN_TOKEN, OWN_ROWS) or plan.own_pieces < 1 or plan.own_pieces > 64 or plan.piece_keys < 1 or not (1 if prefix_len else 0) <= plan.prefix_pieces <= (64 if prefix_len else 0):
         raise KernelError(f"{who}: the plan does not fit a prefix of {prefix_len} keys")
     floats = n * n_q_heads * records * head_dim if records > 1 else 0
     _packed_vector(scratch, "scratch", who, torch.float32, floats + (n * n_q_heads * records * 2 if records > 1 else 0))
@@ -2572,7 +2588,7 @@ def attention_shared_prefix(q: torch.Tensor, k_pages: torch.Tensor, v_pages: tor
     part_o = scratch.data_ptr()
     if plan.tensor_cores and packed_tc_supported(q.dtype, head_dim, n_q_heads // n_kv_heads, page_size) and _on_16_bytes(ld_q | ld_o, q, out, k_pages, v_pages, scratch) \
             and ld_q >= n_q_heads * head_dim and n_pages * n_kv_heads * page_size <= 0x7fffffff:
-        fn, how = _fn("attention_packed_tc", None, "erb_attention_shared_prefix_tc"), (int(plan.prefix_dual), plan.own)
+        fn, how = _fn("attention_packed_tc", None, "erb_attention_shared_prefix_tc"), (plan.own,)
     else:
         fn, how = _fn("attention_packed", _elem(q), "erb_attention_shared_prefix"), ()
     _call(fn, q, ld_q, k_pages, v_pages, n_pages, page_size, prefix_pages, int(prefix_len), block_tables, block_tables.shape[1], seq_starts, positions, n_seqs,

@@ -232,13 +232,12 @@ def test_any_cut_gives_the_same(elem, plan):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dim", [64, 128])
-@pytest.mark.parametrize("plan", [(1, 1, 4096, False), (3, 2, 128, False), (2, 2, 4096, True), (64, 1, 128, True), (6, 64, 128, True), (4, 6, 64, True),
-                                  (2, 3, 256, False), (1, 1, 64, False)])
+@pytest.mark.parametrize("plan", [(1, 1, 4096), (3, 2, 128), (2, 2, 4096), (64, 1, 128), (6, 64, 128), (4, 6, 64), (2, 3, 256), (1, 1, 64)])
 @pytest.mark.parametrize("own", [K.OWN_MANY, K.OWN_TOKEN, K.OWN_ROWS])
 def test_any_cut_gives_the_same_on_tensor_cores(dim, plan, own):
     c = shared_call("bfloat16", 330, (1, 4, 1, 40), (0, 260, 31, 500), 4, 2, dim, 16)
     records = plan[0] + plan[1]
-    out, status = run_shared(c, K.SharedPrefixPlan(*plan[:3], 46 * 4 * records * (dim + 2), True, plan[3], own))
+    out, status = run_shared(c, K.SharedPrefixPlan(*plan, 46 * 4 * records * (dim + 2), True, own))
     assert status == 0
     check_shared(c, out)
 
