@@ -13,6 +13,8 @@
 //
 // Bytes bound it: every entry is read once and written once.  A thread moves 2 V entries that hold whole pairs (V: sixteen bytes of
 // entries), so the lanes of a head exchange nothing but the norm's sum; a token's angles are taken once by the block that works on it.
+// 8,192 tokens of 32 + 8 + 8 heads of 128, bfloat16, into the cache: 38 us, 201 MB read and written, 0.81 of what a copy moves; 2,501 tokens of
+// 15 + 5 heads of 64, float, half of each turned: 6.7 us, 3.8 TB/s.
 #include <stdarg.h>
 
 #include "common.cuh"
@@ -149,10 +151,10 @@ template <> struct Piece<__nv_bfloat16> {
 // Rows on 16-byte boundaries, heads of UNITS * 2 N entries (N: sixteen bytes of entries), turned entries a multiple of 2 N.  A unit is two
 // pieces of sixteen bytes that hold whole pairs: neighbours with `pairs`, else piece u of the first half of the turned part and its partner
 // in the second half (behind the turned part: two neighbours).  UNITS neighbouring lanes make a head.  A block works on the units of one
-// token, kAhead for each thread, asked for before the token's angles are made, blockIdx.y telling apart the blocks that share a token.
-constexpr int kFastThreads = 128, kAhead = 2;
+// token, AHEAD for each thread, asked for before the token's angles are made, blockIdx.y telling apart the blocks that share a token.
+constexpr int kFastThreads = 128;
 
-template <int UNITS, bool PAIRS>
+template <int UNITS, bool PAIRS, int AHEAD>
 __global__ void __launch_bounds__(kFastThreads) rotary_units_kernel(const RotaryArgs a) {
   using P = Piece<elem_t>;
   constexpr int N = P::N, D = UNITS * 2 * N;
@@ -172,10 +174,10 @@ __global__ void __launch_bounds__(kFastThreads) rotary_units_kernel(const Rotary
   const long long cache_row = slot < 0 ? 0 : ((slot / a.page_size) * a.nkv * a.page_size + slot % a.page_size) * D;
   const long long head_step = (long long)a.page_size * D;                // from a kv head's row of a page to the next head's
   bool first = true;
-  for (int w0 = blockIdx.y * kFastThreads; w0 < all; w0 += stride * kAhead) {      // (uniform: the lanes of a head stay together)
-    uint4 x0[kAhead], x1[kAhead];
+  for (int w0 = blockIdx.y * kFastThreads; w0 < all; w0 += stride * AHEAD) {      // (uniform: the lanes of a head stay together)
+    uint4 x0[AHEAD], x1[AHEAD];
 #pragma unroll
-    for (int n = 0; n < kAhead; ++n) {
+    for (int n = 0; n < AHEAD; ++n) {
       const int w = w0 + n * stride + threadIdx.x, head = w / UNITS;
       x0[n] = x1[n] = make_uint4(0, 0, 0, 0);
       if (w >= all) continue;
@@ -190,7 +192,7 @@ __global__ void __launch_bounds__(kFastThreads) rotary_units_kernel(const Rotary
       first = false;
     }
 #pragma unroll
-    for (int n = 0; n < kAhead; ++n) {
+    for (int n = 0; n < AHEAD; ++n) {
       const int w = w0 + n * stride + threadIdx.x, head = w / UNITS;
       if (w0 + n * stride >= all) break;                                 // (the whole block)
       float lo[N], hi[N];
@@ -247,10 +249,26 @@ __global__ void __launch_bounds__(kFastThreads) rotary_units_kernel(const Rotary
   }
 }
 
+// As many blocks a token as its units fill, no more than give each multiprocessor sixteen (8,192 tokens: with 64 43.1 us, with 2 to 32 39.7).
+template <int UNITS, int AHEAD>
+void launch_ahead(const RotaryArgs& a, int work, cudaStream_t stream) {
+  int share = (work + kFastThreads * AHEAD - 1) / (kFastThreads * AHEAD);
+  const int want = (sm_count() * 16 + a.n_tokens - 1) / a.n_tokens;
+  share = share < want ? share : want;
+  const dim3 grid(a.n_tokens, share < 1 ? 1 : share);
+  if (a.pairs) launch_chained(rotary_units_kernel<UNITS, true, AHEAD>, grid, dim3(kFastThreads), 0, stream, a);
+  else launch_chained(rotary_units_kernel<UNITS, false, AHEAD>, grid, dim3(kFastThreads), 0, stream, a);
+}
+// Few tokens: one unit a thread, so that a token's work is in as many blocks as it has (16 tokens of 48 heads of 128, bfloat16: 2.4 us; two
+// units 2.6, three 2.9; 128 tokens 2.7 and 2.8; but 256 3.8 and 3.3).  Many: a token's units in one block where it can, its angles made once
+// (1,024 tokens of 48 heads: three 6.2 us, two 6.9; 8,192 38.6 and 39.8), and no more than it needs (8,192 tokens of 25 heads of 64: two 12.9 us,
+// three 14.2: registers).
 template <int UNITS>
-void launch_units(const RotaryArgs& a, dim3 grid, cudaStream_t stream) {
-  if (a.pairs) launch_chained(rotary_units_kernel<UNITS, true>, grid, dim3(kFastThreads), 0, stream, a);
-  else launch_chained(rotary_units_kernel<UNITS, false>, grid, dim3(kFastThreads), 0, stream, a);
+void launch_units(const RotaryArgs& a, int work, cudaStream_t stream) {
+  const long long blocks = (long long)a.n_tokens * ((work + kFastThreads - 1) / kFastThreads);
+  if (blocks <= 3LL * sm_count()) launch_ahead<UNITS, 1>(a, work, stream);
+  else if (work <= 2 * kFastThreads) launch_ahead<UNITS, 2>(a, work, stream);
+  else launch_ahead<UNITS, 3>(a, work, stream);
 }
 
 }  // namespace
@@ -278,17 +296,12 @@ ERB_EXPORT int erb_rotary_append(const void* q, void* q_out, long long ld_q, lon
   if (head_dim % (2 * N) == 0 && rot_dim % (2 * N) == 0 && units >= 2 && units <= 32 && !(units & (units - 1)) && !(all & 15) &&
       !((ld_q | ld_qo | ld_k | ld_ko | ld_v) % N)) {
     const int work = (nq + (k ? nkv : 0) + (v ? nkv : 0)) * units;
-    // As many blocks a token as its units fill, no more than give each multiprocessor sixteen.
-    int share = (work + kFastThreads * kAhead - 1) / (kFastThreads * kAhead);
-    const int want = (sm_count() * 16 + n_tokens - 1) / n_tokens;
-    share = share < want ? share : want;
-    const dim3 grid(n_tokens, share < 1 ? 1 : share);
     switch (units) {
-      case 2: launch_units<2>(a, grid, (cudaStream_t)stream); break;
-      case 4: launch_units<4>(a, grid, (cudaStream_t)stream); break;
-      case 8: launch_units<8>(a, grid, (cudaStream_t)stream); break;
-      case 16: launch_units<16>(a, grid, (cudaStream_t)stream); break;
-      default: launch_units<32>(a, grid, (cudaStream_t)stream);
+      case 2: launch_units<2>(a, work, (cudaStream_t)stream); break;
+      case 4: launch_units<4>(a, work, (cudaStream_t)stream); break;
+      case 8: launch_units<8>(a, work, (cudaStream_t)stream); break;
+      case 16: launch_units<16>(a, work, (cudaStream_t)stream); break;
+      default: launch_units<32>(a, work, (cudaStream_t)stream);
     }
     return check_launch("rotary_append");
   }

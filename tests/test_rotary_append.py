@@ -50,6 +50,10 @@ CASES = [
     (9, 4, 1, 96, 96, True, 2.0, False, 123456, 0, 5),
     (300, 8, 8, 64, 16, False, 1.0, False, 4000, 64, 0),
     (2, 2, 2, 1024, 1024, False, 1.0, True, 5, 4, 0),
+    (470, 32, 8, 128, 128, False, 1.0, True, 5, 16, 0),
+    (460, 6, 2, 64, 32, True, 1.2, True, 90000, 8, 8),
+    (500, 64, 8, 128, 64, False, 1.0, True, 3, 32, 0),
+    (2500, 20, 6, 128, 32, False, 1.1, False, 0, 16, 0),
 ]
 
 
