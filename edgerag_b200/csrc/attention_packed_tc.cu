@@ -30,6 +30,11 @@
 // that is no number would spoil rows that do not see it; so the values of such tiles are looked over before they are used: rows of V that
 // nobody sees become zeros, and an infinity or NaN that only some rows see becomes zero and is added to exactly those rows at the end.
 //
+// What bounds it: a half step's chain, scores -> softmax -> P V, that two query tiles only partly hide from each other (polynomial exponentials,
+// sixteen softmax warps and smaller chunks of P made it slower), and the tail of uneven pieces.  8,192 tokens, 32 query heads on 8 of 128: 486 us,
+// 1.13 PFLOP/s, 0.68 of a library product's rate (one tile of 128 keys at a time 545 us, one issuing warp 583, a block for each piece 700;
+// CUDA cores 20,650).  23 prompts of up to 2,001 tokens, 32 heads of 64: 150 us.  1 to 64 rows behind 16,384 keys: 24 to 60 us, 2.8 TB/s.
+//
 // Every wait is bounded: a thread that gives up raises a block-wide flag, every other wait of the block then ends too, the block records a
 // code in *status, lets its copies land, frees its TMEM and returns.
 #include <limits.h>
