@@ -51,8 +51,7 @@ __device__ __forceinline__ void copy16(float* dst, const void* src, bool real) {
 }
 
 template <int DMAX, int MODE>
-__global__ void __launch_bounds__(kThreads) attention_packed_kernel(const PackedArgs a, const int wide) {
-  chain_wait();
+__device__ __forceinline__ void work_on(const PackedArgs& a, const int wide) {
   extern __shared__ __align__(16) uint8_t raw[];
   Smem<DMAX>& sm = *reinterpret_cast<Smem<DMAX>*>(raw);
   constexpr int LD = Smem<DMAX>::kLd, LDP = Smem<DMAX>::kLdP, NC = DMAX / 64;
@@ -306,6 +305,14 @@ __global__ void __launch_bounds__(kThreads) attention_packed_kernel(const Packed
 }
 
 template <int DMAX, int MODE>
+__global__ void __launch_bounds__(kThreads) attention_packed_kernel(const PackedArgs a, const int wide) {
+  const bool early = MODE == kOwn && a.early;
+  if (!early) chain_wait();
+  work_on<DMAX, MODE>(a, wide);
+  if (early) chain_wait();         // (a kernel after this one may count on the one over the prefix being done, too)
+}
+
+template <int DMAX, int MODE>
 int launch_tiles(const PackedArgs& a, dim3 grid, cudaStream_t stream, const char* who) {
   const int bytes = (int)sizeof(Smem<DMAX>);
   static bool configured[64] = {};
@@ -383,6 +390,7 @@ ERB_EXPORT int erb_attention_shared_prefix(const void* q, long long ld_q, const 
   }
   a.rec0 = prefix_len > 0 ? prefix_pieces : 0;
   a.pieces = own_pieces;
+  a.early = prefix_len > 0;
   const int rc = launch_by_size<kOwn>(a, dim3((unsigned)(n_seqs * own_pieces), nkv, 1), s, "attention_shared_prefix");
   if (rc || n_rec <= 1) return rc;
   return launch_merge(a, s, "attention_shared_prefix");

@@ -172,7 +172,8 @@ attention_packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
   __syncthreads();
   fence_after_sync();
   const uint32_t tmem = *s_tmem;
-  chain_wait();
+  const bool early = MODE == kOwn && a.early;
+  if (!early) chain_wait();
 
   bool ok = true;                        // the same for a whole warp
   auto wait = [&](int which, int phase) {
@@ -654,6 +655,7 @@ attention_packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
     fence_after_sync();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
   }
+  if (early) chain_wait();         // (a kernel after this one may count on the one over the prefix being done, too)
 }
 
 // A tensor map over the queries [tokens][heads][D], boxes of 64 columns, the G heads of a kv head and as many whole tokens as 128 rows hold.
@@ -784,6 +786,7 @@ ERB_EXPORT int erb_attention_shared_prefix_tc(const void* q, long long ld_q, con
   }
   a.rec0 = prefix_len > 0 ? prefix_pieces : 0;
   a.pieces = own_pieces;
+  a.early = prefix_len > 0;
   if (own == kOwnMany) {
     if ((rc = launch_tc<kOwn>(a, mk, mv, (rows / rows_of_piece(nq / nkv) + n_seqs) * nkv * a.pieces, s, who)) || n_rec <= 1) return rc;
   } else {

@@ -41,6 +41,7 @@ struct PackedArgs {
   float *part_o, *part_ml;         // records: [(token * nq + head) * n_rec + piece]
   int n_rec, rec0, pieces;         // records of a row, the first of this call's pieces, how many pieces it cuts the keys into
   int piece_keys;                  // kOwn: keys of a piece (the last one takes the rest)
+  int early;                       // kOwn behind a kernel over the prefix: may run beside it (all that is read was complete when that one began)
   int* status;
 };
 
