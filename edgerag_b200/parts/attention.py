@@ -36,7 +36,7 @@ tensor ``vmix``).
 With positions scaled for long contexts (``rope_scaled``) the norm per head, the rotation and the cache write are one kernel
 (``kernels.rotary_append``).  ``whole_prompts``: where every portion of a step is its prompt's beginning, keys and values are taken from the step's
 rows instead of the cache (``kernels.attention_prompt``: tensor cores for heads of 64 and 128); positions then have to be scaled ones or none,
-since only those leave the rows' keys as the cache has them.
+since only those leave the rows' keys as the cache has them.  A call that reads the cache another call wrote takes its keys from there.
 
 Heads whose sizes differ or are no multiple of 8 are stored padded with zeros to one size ``D``:
 scores and outputs are unchanged, and the norm's mean divides by the true count.
@@ -240,8 +240,9 @@ class Attention(Mixer):
         if self.qk_norm_eps is not None:
             self.q_norm, self.k_norm = f32(tensors[nm["q_norm"]]), f32(tensors[nm["k_norm"]])
 
-    def _prepare(self, x, qkv, ctx, pages, slots) -> None:
-        """The input product and everything between it and the attention: biases, head norms, positions, cache write."""
+    def _prepare(self, x, qkv, ctx, pages, slots, keys_stay=False) -> None:
+        """The input product and everything between it and the attention: biases, head norms, positions, cache write.
+        ``keys_stay``: the attention reads the rows' keys, too."""
         d = self.head_dim
         if self.whole:
             pos = self.position
@@ -262,7 +263,7 @@ class Attention(Mixer):
         if self.scaled:
             kernels.linear(x, self.w_qkv, qkv)
             self.position.prepare(qkv, ctx, self.n_q, self.n_kv, d, pages, slots, self.q_norm, self.k_norm, self.qk_norm_eps or 0.0,
-                                  keys_stay=self.whole_prompts and ctx.whole_portions and ctx.n_tokens > ctx.n_decode)
+                                  keys_stay=keys_stay)
             return
         if self.qk_bias or self.qk_norm_eps is not None or self.values_are_keys:
             pos = self.position
@@ -286,6 +287,8 @@ class Attention(Mixer):
         group = ctx.group_of(call.cache_layer)
         write = call.writes_cache and self.own_kv
         pages, slots = ((k_pages, v_pages), ctx.slots[group]) if write else (None, None)
+        # keys and values are all in the step's rows (a call that reads another call's cache has none of its own there)
+        from_rows = write and self.whole_prompts and ctx.whole_portions and n > ctx.n_decode
         if self.conv_form:      # queries into rows of their own: a row's convolution reads the rows before it
             kernels.linear(x, self.w_qkv, qkv)
             q = ctx.buf("attn.q", (n, self.q_width), self.dtype)
@@ -295,7 +298,7 @@ class Attention(Mixer):
                              first_portion=ctx.n_decode, slots=slots, k_pages=k_pages, v_pages=v_pages, page_size=ctx.page_size)
             qkv = q
         else:
-            self._prepare(x, qkv, ctx, pages, slots)
+            self._prepare(x, qkv, ctx, pages, slots, from_rows)
         out = ctx.buf("attn.out", (n, self.q_width), self.dtype)
         gate = None if self.gate_name is None else qkv[:, self.gate_off: self.gate_off + self.q_width]
         score = {"penalty": self.penalty, "softcap": self.softcap}
@@ -355,7 +358,7 @@ class Attention(Mixer):
                                          out_rows, self.n_q, self.scale, part_acc, part_ml, max_splits,
                                          window=self.window, split_keys=split, keep_first=self.keep_first, chunk=self.chunk,
                                          gate=head_gate, **score)
-        if n > nd and self.whole_prompts and ctx.whole_portions:        # keys and values are all in the step's rows
+        if from_rows:
             q, k, v = qkv[:, : self.q_width], qkv[:, self.q_width: self.q_width + self.kv_width], qkv[:, self.q_width + self.kv_width:]
             kernels.attention_prompt(q, k, v, ctx.seq_starts[nd:], out, self.n_q, self.n_kv, self.scale, ctx.status)
         elif n > nd and kernels.prefill_tc_supported(self.dtype, d, self.window, ctx.page_size):
