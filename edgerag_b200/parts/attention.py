@@ -36,7 +36,8 @@ tensor ``vmix``).
 With positions scaled for long contexts (``rope_scaled``) the norm per head, the rotation and the cache write are one kernel
 (``kernels.rotary_append``).  ``whole_prompts``: where every portion of a step is its prompt's beginning, keys and values are taken from the step's
 rows instead of the cache (``kernels.attention_prompt``: tensor cores for heads of 64 and 128); positions then have to be scaled ones or none,
-since only those leave the rows' keys as the cache has them.  A call that reads the cache another call wrote takes its keys from there.
+since only those leave the rows' keys as the cache has them.  A call that reads the cache another call wrote takes its keys from there, and
+with ``EngineOptions.batch_invariant`` every portion does: another request's portion with a past would otherwise change a prompt's kernel.
 
 Heads whose sizes differ or are no multiple of 8 are stored padded with zeros to one size ``D``:
 scores and outputs are unchanged, and the norm's mean divides by the true count.
@@ -287,8 +288,9 @@ class Attention(Mixer):
         group = ctx.group_of(call.cache_layer)
         write = call.writes_cache and self.own_kv
         pages, slots = ((k_pages, v_pages), ctx.slots[group]) if write else (None, None)
-        # keys and values are all in the step's rows (a call that reads another call's cache has none of its own there)
-        from_rows = write and self.whole_prompts and ctx.whole_portions and n > ctx.n_decode
+        # keys and values are all in the step's rows (a call that reads another call's cache has none of its own there; whether every portion
+        # begins its prompt is a matter of the whole step, so pinned launch shapes leave the rows alone)
+        from_rows = write and self.whole_prompts and ctx.whole_portions and not ctx.batch_invariant and n > ctx.n_decode
         if self.conv_form:      # queries into rows of their own: a row's convolution reads the rows before it
             kernels.linear(x, self.w_qkv, qkv)
             q = ctx.buf("attn.q", (n, self.q_width), self.dtype)

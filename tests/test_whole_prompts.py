@@ -89,3 +89,32 @@ def test_a_layer_called_twice_reads_its_own_cache(position, dtype):
     for portions in ([[70], [33], [5]], [[40, 30], [1] * 33, [5]]):
         for a, b in zip(walk(cached, SEQUENCES, portions), walk(rows, SEQUENCES, portions)):
             assert (a - b).abs().max() <= (2e-4 + 2e-4 * a.abs().max() if dtype == torch.float32 else 0.02 * a.abs().max())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("position", POSITIONS)
+def test_pinned_launch_shapes_do_not_look_at_other_requests(position, dtype, monkeypatch):
+    """`batch_invariant`: whether another request's portion has a past does not change the kernel that takes a prompt."""
+    seen = [[c[0] for c in launches(monkeypatch, POSITIONS[position], LayerCall(0, 0), dtype, True, whole)] for whole in (True, False)]
+    assert seen[0] == seen[1] and "attention_prompt" not in seen[0]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("position", POSITIONS)
+def test_a_prompt_has_its_bits_whatever_shares_its_step(position):
+    """32-bit portions under `batch_invariant`: beside another prompt, and beside as many tokens of another one's second portion (the products
+    of the two steps have the same shapes)."""
+    from edgerag_b200.engine.step import StepEntry
+
+    runner = build(torch.float32, POSITIONS[position], True, [LayerCall(0, 0), LayerCall(1, 1)], batch_invariant=True)
+    prompt, other, got = SEQUENCES[0], SEQUENCES[1], []
+    for parts in ((other[:20],), (other[:13], other[13:])):
+        for name in ("a", "b"):
+            runner.admit(name)
+        for part in parts[:-1]:
+            runner.step([StepEntry("b", tokens=list(part), want=[0])])
+        step = [StepEntry("a", tokens=list(prompt), want=list(range(len(prompt)))), StepEntry("b", tokens=list(parts[-1]), want=[0])]
+        got.append(runner.step(step)[: len(prompt)].float().cpu().clone())
+        for name in ("a", "b"):
+            runner.release(name)
+    assert torch.equal(got[0], got[1])
