@@ -49,6 +49,8 @@ edgerag/cache/paged.py:208-238).
 
 from __future__ import annotations
 
+import math
+
 import torch
 
 from ..cache.manager import KVGroupSpec, StateSpec
@@ -124,6 +126,8 @@ class Attention(Mixer):
                                    or (qk_norm_eps is not None and not self.scaled)):
             raise ValueError("attention: whole prompts are taken from their rows: keys of the layer's own, positions scaled or none, and no other option "
                              "than a norm per head with scaled positions")
+        if self.whole_prompts and (head_dim > 256 or not (math.isfinite(self.scale) and self.scale > 0)):
+            raise ValueError(f"attention: whole prompts take heads of up to 256 and a positive scale, not {head_dim} and {self.scale}")
         self.q_width = n_q_heads * head_dim
         self.kv_width = n_kv_heads * head_dim
         self.in_width = self.q_width + (1 if self.values_are_keys else 2) * self.kv_width

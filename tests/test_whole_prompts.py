@@ -118,3 +118,13 @@ def test_a_prompt_has_its_bits_whatever_shares_its_step(position):
         for name in ("a", "b"):
             runner.release(name)
     assert torch.equal(got[0], got[1])
+
+
+@pytest.mark.parametrize("how,word", [({"head_dim": 272}, "256"), ({"scale": 0.0}, "scale"), ({"scale": -0.125}, "scale"), ({"scale": float("nan")}, "scale")])
+def test_what_the_first_prompt_would_refuse_is_refused_at_once(how, word):
+    """Head sizes and scales that attention over rows does not take."""
+    make = lambda **more: attention.Attention(**{"hidden": 64, "n_q_heads": 4, "n_kv_heads": 2, "head_dim": 64, "position": PartSpec("none"),   # noqa: E731
+                                                 "dtype": torch.float32, "device": torch.device("cpu"), **how, **more})
+    make()
+    with pytest.raises(ValueError, match=word):
+        make(whole_prompts=True)
