@@ -19,6 +19,9 @@
 
 namespace erb {
 
+// Keys of a piece: an int still holds them when they are rounded up to tiles.
+constexpr int kMostPieceKeys = 1 << 30;
+
 constexpr int kPrompt = 0, kPrefix = 1, kOwn = 2;
 
 // Codes of the status word beside those of waits: a page that lies outside the pool, sequences that do not lie inside the rows.

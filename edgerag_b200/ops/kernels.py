@@ -2468,6 +2468,7 @@ class SharedPrefixPlan(NamedTuple):
 
 
 OWN_MANY, OWN_TOKEN, OWN_ROWS = 0, 1, 2
+_MOST_PIECE_KEYS = 1 << 30       # (an int still holds them when they are rounded up to tiles)
 
 
 def _cut(tiles: int, blocks: int, sms: int, fixed: int) -> int:
@@ -2519,12 +2520,12 @@ def shared_prefix_plan(n_tokens: int, n_seqs: int, n_q_heads: int, n_kv_heads: i
         if own == OWN_MANY:
             tiles = own_keys // 128 + 2 - (prefix_len % 128 == 0)
             cut = _cut(tiles, max(1, n_kv_heads * max(n_seqs, -(-n_tokens * group // (2 * tile)))), sms, 3)
-            piece_keys = -(-tiles // cut) * 128
+            piece_keys = min(-(-tiles // cut) * 128, _MOST_PIECE_KEYS)
             prefix_pieces = _cut(-(-prefix_len // 128), prefix_blocks, sms, 4) if prefix_len else 0
         else:       # small blocks, four a multiprocessor; with one piece there is no separate merge
             blocks = n_kv_heads * max(1, n_seqs if own == OWN_TOKEN else -(-n_tokens * group // 64))
             cut = min(max(1, 4 * sms // blocks), max(1, own_keys // 512), 64)
-            piece_keys = -(-own_keys // (64 * cut)) * 64
+            piece_keys = min(-(-own_keys // (64 * cut)) * 64, _MOST_PIECE_KEYS)
             prefix_pieces = _cut_prefix(-(-prefix_len // 128), prefix_blocks, blocks * cut, sms) if prefix_len else 0
         own_pieces = max(1, -(-(tiles * 128 if own == OWN_MANY else own_keys) // piece_keys))
         records = prefix_pieces + own_pieces
@@ -2535,7 +2536,7 @@ def shared_prefix_plan(n_tokens: int, n_seqs: int, n_q_heads: int, n_kv_heads: i
     tiles = -(-prefix_len // 64)
     prefix_pieces = min(max(1, 2 * sms // blocks), max(1, tiles // 2), 64) if prefix_len else 0
     own_pieces = min(max(1, 2 * sms // max(1, n_seqs * n_kv_heads)), max(1, own_keys // 128), 64)
-    piece_keys = -(-own_keys // (64 * own_pieces)) * 64
+    piece_keys = min(-(-own_keys // (64 * own_pieces)) * 64, _MOST_PIECE_KEYS)
     own_pieces = -(-own_keys // piece_keys)
     records = prefix_pieces + own_pieces
     floats = n_tokens * n_q_heads * records * (head_dim + 2) if records > 1 else 0
@@ -2579,7 +2580,8 @@ def attention_shared_prefix(q: torch.Tensor, k_pages: torch.Tensor, v_pages: tor
     if n * (n_q_heads // n_kv_heads) >= 1 << 30 or n_seqs >= 1 << 24:
         raise KernelError(f"{who}: {n} tokens of {n_q_heads} heads in one call")
     records = plan.prefix_pieces + plan.own_pieces
-    if (plan.own == OWN_TOKEN and n_q_heads // n_kv_heads > 16) or plan.own not in (OWN_MANY, OWN_TOKEN, OWN_ROWS) or plan.own_pieces < 1 or plan.own_pieces > 64 or plan.piece_keys < 1 or not (1 if prefix_len else 0) <= plan.prefix_pieces <= (64 if prefix_len else 0):
+    if (plan.own == OWN_TOKEN and n_q_heads // n_kv_heads > 16) or plan.own not in (OWN_MANY, OWN_TOKEN, OWN_ROWS) or not 1 <= plan.own_pieces <= 64 or not 1 <= plan.piece_keys <= _MOST_PIECE_KEYS \
+            or not (1 if prefix_len else 0) <= plan.prefix_pieces <= (64 if prefix_len else 0):
         raise KernelError(f"{who}: the plan does not fit a prefix of {prefix_len} keys")
     floats = n * n_q_heads * records * head_dim if records > 1 else 0
     _packed_vector(scratch, "scratch", who, torch.float32, floats + (n * n_q_heads * records * 2 if records > 1 else 0))

@@ -1,0 +1,29 @@
+"""Sizes at which a count in an int, or the arithmetic on it, would overflow: refused before anything is launched (CPU)."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from edgerag_b200.ops import kernels as K
+from test_packed_attention import PAGED
+
+
+@pytest.mark.parametrize("piece_keys", [2**30 + 1, 2**31 - 127, 2**31 - 1, 2**32 + 64])
+@pytest.mark.parametrize("plan", [(1, 1), (2, 3)])
+def test_pieces_that_their_arithmetic_cannot_hold_are_refused(plan, piece_keys):
+    """Rounded up to tiles, pieces of almost 2^31 keys were negative ones, and the last of several then walked tiles from far before the first key on."""
+    for tensor_cores in (True, False):
+        records = sum(plan)
+        made = K.SharedPrefixPlan(*plan, piece_keys, 6 * 4 * records * 66, tensor_cores)
+        with pytest.raises(K.KernelError, match="plan does not fit"):
+            K.attention_shared_prefix(**{**PAGED, "plan": made, "scratch": torch.zeros(made.floats)})
+
+
+@pytest.mark.parametrize("nq,nkv,dim,rows,fresh", [(32, 8, 128, 64, 1), (32, 8, 128, 6400, 100), (4, 2, 80, 6400, 100), (512, 512, 64, 600, 4), (2, 1, 64, 1, 1)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("keys", [2**30 + 5, 2**31 - 257, 2**31 - 1])
+def test_plans_for_the_longest_contexts_stay_within_that(nq, nkv, dim, rows, fresh, dtype, keys):
+    for prefix in (0, 77, 4096):
+        p = K.shared_prefix_plan(rows, rows // fresh, nq, nkv, dim, dtype, 16, prefix, keys, fresh, sms=148)
+        assert p.piece_keys <= 2**30 and 1 <= p.own_pieces <= 64 and p.own_pieces * p.piece_keys >= keys - prefix
