@@ -368,7 +368,8 @@ ERB_EXPORT int erb_attention_shared_prefix(const void* q, long long ld_q, const 
                                            float* part_ml, int* status, void* stream) {
   if (n_seqs <= 0 || n_tokens <= 0) return ERB_OK;
   if (nq <= 0 || nkv <= 0 || nq % nkv || head_dim <= 0 || head_dim > 256 || !status || n_pages <= 0 || page_size <= 0 || prefix_len < 0 ||
-      table_ld <= 0 || prefix_pieces < (prefix_len > 0 ? 1 : 0) || own_pieces < 1 || piece_keys <= 0 || piece_keys > kMostPieceKeys)
+      table_ld <= 0 || prefix_pieces < (prefix_len > 0 ? 1 : 0) || own_pieces < 1 || piece_keys <= 0 || piece_keys > kMostPieceKeys ||
+      prefix_len > kMostKeys || (long long)table_ld * page_size > kMostKeys)
     return fail(ERB_ERR_ARG, "attention_shared_prefix: bad sizes");
   const int n_rec = (prefix_len > 0 ? prefix_pieces : 0) + own_pieces;
   if (n_rec > 1 && (!part_o || !part_ml)) return fail(ERB_ERR_ARG, "attention_shared_prefix: pieces need scratch");

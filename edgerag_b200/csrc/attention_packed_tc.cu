@@ -757,7 +757,8 @@ ERB_EXPORT int erb_attention_shared_prefix_tc(const void* q, long long ld_q, con
                                               float* part_o, float* part_ml, int* status, void* stream) {
   if (n_seqs <= 0 || n_tokens <= 0) return ERB_OK;
   if (nq <= 0 || nkv <= 0 || nq % nkv || !status || n_pages <= 0 || prefix_len < 0 || table_ld <= 0 || prefix_pieces < (prefix_len > 0 ? 1 : 0) ||
-      own_pieces < 1 || piece_keys <= 0 || piece_keys > kMostPieceKeys || !(scale > 0.f) || prefix_pieces > 64 ||
+      own_pieces < 1 || piece_keys <= 0 || piece_keys > kMostPieceKeys || prefix_len > kMostKeys || (long long)table_ld * page_size > kMostKeys ||
+      !(scale > 0.f) || prefix_pieces > 64 ||
       own < kOwnMany || own > kOwnRows || (own == kOwnToken && nq / nkv > 16))
     return fail(ERB_ERR_ARG, "attention_shared_prefix_tc: bad sizes");
   if ((head_dim != 64 && head_dim != 128) || nq / nkv > BM || !aligned(q, ld_q) || !aligned(out, ld_out) || !aligned(k_pages, 0) || !aligned(v_pages, 0) ||

@@ -19,6 +19,8 @@
 
 namespace erb {
 
+// Keys of a context: the tile that holds the last one (of up to 128) and the one asked for ahead of it end inside an int.
+constexpr int kMostKeys = 0x7fffffff - 255;
 // Keys of a piece: an int still holds them when they are rounded up to tiles.
 constexpr int kMostPieceKeys = 1 << 30;
 

@@ -2468,6 +2468,7 @@ class SharedPrefixPlan(NamedTuple):
 
 
 OWN_MANY, OWN_TOKEN, OWN_ROWS = 0, 1, 2
+_MOST_KEYS = (1 << 31) - 256      # of a context: the tile that holds the last one ends inside an int
 _MOST_PIECE_KEYS = 1 << 30       # (an int still holds them when they are rounded up to tiles)
 
 
@@ -2568,13 +2569,15 @@ def attention_shared_prefix(q: torch.Tensor, k_pages: torch.Tensor, v_pages: tor
     if k_pages.shape != v_pages.shape or k_pages.dtype != q.dtype or v_pages.dtype != q.dtype or not k_pages.is_contiguous() or not v_pages.is_contiguous() \
             or n_pages * page_size == 0:
         raise KernelError(f"{who}: pools must be contiguous, of one shape and of q's type")
-    if prefix_len < 0 or prefix_len > 0x7fffffff - page_size:
+    if not 0 <= prefix_len <= _MOST_KEYS:
         raise KernelError(f"{who}: prefix of {prefix_len} keys")
     _packed_vector(prefix_pages, "prefix_pages", who, torch.int32, -(-prefix_len // page_size))
     _packed_vector(seq_starts, "seq_starts", who, torch.int32, 1)
     n_seqs = seq_starts.numel() - 1
     if block_tables.dim() != 2 or block_tables.dtype != torch.int32 or block_tables.shape[0] < n_seqs or block_tables.shape[1] < 1 or not block_tables.is_contiguous():
         raise KernelError(f"{who}: block_tables must be contiguous int32 [requests, entries]")
+    if block_tables.shape[1] * page_size > _MOST_KEYS:
+        raise KernelError(f"{who}: tables of {block_tables.shape[1] * page_size} keys (at most {_MOST_KEYS})")
     _packed_vector(positions, "positions", who, torch.int32, n)
     _packed_vector(status, "status", who, torch.int32, 1)
     if n * (n_q_heads // n_kv_heads) >= 1 << 30 or n_seqs >= 1 << 24:

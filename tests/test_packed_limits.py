@@ -27,3 +27,16 @@ def test_plans_for_the_longest_contexts_stay_within_that(nq, nkv, dim, rows, fre
     for prefix in (0, 77, 4096):
         p = K.shared_prefix_plan(rows, rows // fresh, nq, nkv, dim, dtype, 16, prefix, keys, fresh, sms=148)
         assert p.piece_keys <= 2**30 and 1 <= p.own_pieces <= 64 and p.own_pieces * p.piece_keys >= keys - prefix
+
+
+def test_contexts_that_a_walk_cannot_end_are_refused():
+    """A walk whose last tile ends behind 2^31 - 1 would start again from below zero: the longest context and prefix lie a tile before that."""
+    pools = {x: torch.empty(1, 2, 1 << 16, 64) for x in ("k_pages", "v_pages")}
+    wide = {**PAGED, **pools, "prefix_len": 40, "prefix_pages": torch.zeros(1, dtype=torch.int32)}
+    for entries, word in ((2**15 - 1, "CUDA device"), (2**15, "keys")):
+        with pytest.raises(K.KernelError, match=word):
+            K.attention_shared_prefix(**{**wide, "block_tables": torch.empty(6, entries, dtype=torch.int32)})
+    pages = torch.empty(2**27, dtype=torch.int32)                     # (never touched)
+    for prefix, word in ((2**31 - 256, "CUDA device"), (2**31 - 255, "prefix of"), (2**31 - 17, "prefix of"), (2**32 + 40, "prefix of")):
+        with pytest.raises(K.KernelError, match=word):
+            K.attention_shared_prefix(**{**PAGED, "prefix_len": prefix, "prefix_pages": pages})
