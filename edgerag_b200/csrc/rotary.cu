@@ -253,7 +253,7 @@ __global__ void __launch_bounds__(kFastThreads) rotary_units_kernel(const Rotary
 template <int UNITS, int AHEAD>
 void launch_ahead(const RotaryArgs& a, int work, cudaStream_t stream) {
   int share = (work + kFastThreads * AHEAD - 1) / (kFastThreads * AHEAD);
-  const int want = (sm_count() * 16 + a.n_tokens - 1) / a.n_tokens;
+  const int want = (int)((sm_count() * 16LL + a.n_tokens - 1) / a.n_tokens);
   share = share < want ? share : want;
   const dim3 grid(a.n_tokens, share < 1 ? 1 : share);
   if (a.pairs) launch_chained(rotary_units_kernel<UNITS, true, AHEAD>, grid, dim3(kFastThreads), 0, stream, a);

@@ -2304,6 +2304,12 @@ def _packed_vector(t: torch.Tensor | None, name: str, who: str, dtype: torch.dty
         raise KernelError(f"{who}: {name} must be contiguous {dtype} with at least {at_least} entries")
 
 
+def _in_an_int(who: str, what: str, *counts: int) -> None:
+    """The kernels take these as ints."""
+    if max(counts) > 0x7fffffff:
+        raise KernelError(f"{who}: {max(counts)} {what} (at most {0x7fffffff})")
+
+
 def _on_this_device(who: str, *tensors: torch.Tensor | None) -> None:
     """Every tensor on the current CUDA device: that is where the launch goes."""
     if _host and tensors[0].is_cuda and _host.here(torch._C._cuda_getDevice(), *tensors):
@@ -2352,6 +2358,7 @@ def rotary_append(q: torch.Tensor, positions: torch.Tensor, turns: torch.Tensor 
     if n_q_heads <= 0 or n_kv_heads < 0 or not 0 < head_dim <= 1024:
         raise KernelError(f"{who}: heads {n_q_heads} / {n_kv_heads} of {head_dim} (at most 1024)")
     n, kw = q.shape[0], n_kv_heads * head_dim
+    _in_an_int(who, "tokens", n)
     ld_q = _packed_rows(q, "q", who, n, n_q_heads * head_dim, q.dtype, written=q_out is None)
     ld_qo = ld_q if q_out is None else _packed_rows(q_out, "q_out", who, n, n_q_heads * head_dim, q.dtype, written=True)
     ld_k = ld_ko = ld_v = kw
@@ -2387,6 +2394,7 @@ def rotary_append(q: torch.Tensor, positions: torch.Tensor, turns: torch.Tensor 
             raise KernelError(f"{who}: page layout is not contiguous [pages, kv heads, page_size, head_dim]")
         if n_pages * page_size == 0:
             raise KernelError(f"{who}: the pool has no page")
+        _in_an_int(who, "pages, or tokens of a page", n_pages, page_size)
         ld_v = _packed_rows(v, "v", who, n, kw, q.dtype)
         if n:
             _packed_vector(slots, "slots", who, torch.int32, n)
@@ -2441,6 +2449,7 @@ def attention_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seq_star
     ld_v = _packed_rows(v, "v", who, n, n_kv_heads * head_dim, q.dtype)
     ld_o = _packed_rows(out, "out", who, n, n_q_heads * head_dim, q.dtype, written=True)
     _packed_vector(seq_starts, "seq_starts", who, torch.int32, 1)
+    _in_an_int(who, "sequences", seq_starts.numel() - 1)
     _packed_vector(status, "status", who, torch.int32, 1)
     if n * (n_q_heads // n_kv_heads) >= 1 << 30:
         raise KernelError(f"{who}: {n} tokens of {n_q_heads} heads in one call")
@@ -2569,6 +2578,7 @@ def attention_shared_prefix(q: torch.Tensor, k_pages: torch.Tensor, v_pages: tor
     if k_pages.shape != v_pages.shape or k_pages.dtype != q.dtype or v_pages.dtype != q.dtype or not k_pages.is_contiguous() or not v_pages.is_contiguous() \
             or n_pages * page_size == 0:
         raise KernelError(f"{who}: pools must be contiguous, of one shape and of q's type")
+    _in_an_int(who, "pages", n_pages)
     if not 0 <= prefix_len <= _MOST_KEYS:
         raise KernelError(f"{who}: prefix of {prefix_len} keys")
     _packed_vector(prefix_pages, "prefix_pages", who, torch.int32, -(-prefix_len // page_size))

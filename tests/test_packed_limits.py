@@ -40,3 +40,22 @@ def test_contexts_that_a_walk_cannot_end_are_refused():
     for prefix, word in ((2**31 - 256, "CUDA device"), (2**31 - 255, "prefix of"), (2**31 - 17, "prefix of"), (2**32 + 40, "prefix of")):
         with pytest.raises(K.KernelError, match=word):
             K.attention_shared_prefix(**{**PAGED, "prefix_len": prefix, "prefix_pages": pages})
+
+
+def test_counts_that_an_int_cannot_hold_are_refused():
+    """The kernels take rows, sequences, pages and their sizes as ints: 2^32 + 5 rows would be five.  (Tensors without memory: sizes are all that is looked at.)"""
+    empty = lambda *shape, dtype=torch.bfloat16: torch.empty(shape, dtype=dtype, device="meta")       # noqa: E731
+    ints = lambda *shape: empty(*shape, dtype=torch.int32)                                             # noqa: E731
+    turned = lambda n, **more: K.rotary_append(empty(n, 8), ints(n), None, 1, 1, 8, **more)             # noqa: E731
+    appended = lambda pages, size: turned(4, k=empty(4, 8), v=empty(4, 8), slots=ints(4), k_pages=empty(pages, 1, size, 8),      # noqa: E731
+                                          v_pages=empty(pages, 1, size, 8), status=ints(1))
+    prompt = lambda sequences: K.attention_prompt(empty(6, 256), empty(6, 128), empty(6, 128), ints(sequences + 1), empty(6, 256), 4, 2, 0.125, ints(1))   # noqa: E731
+    behind = lambda pages: K.attention_shared_prefix(empty(6, 256), empty(pages, 2, 16, 64), empty(pages, 2, 16, 64), ints(3), 40, ints(6, 4), ints(7),      # noqa: E731
+                                                     ints(6), empty(6, 256), 4, 0.125, K.SharedPrefixPlan(1, 1, 64, 6 * 4 * 2 * 66), empty(6 * 4 * 2 * 66, dtype=torch.float32), ints(1))
+    for call, fits, word in ((turned, 2**31 - 1, "tokens"), (lambda n: appended(n, 16), 2**31 - 1, "pages"), (lambda n: appended(3, n), 2**31 - 1, "pages"),
+                             (prompt, 2**31 - 1, "sequences"), (behind, 2**31 - 1, "pages")):
+        with pytest.raises(K.KernelError, match="CUDA device"):
+            call(fits)
+        for n in (2**31, 2**32 + 5):
+            with pytest.raises(K.KernelError, match=f"at most 2147483647.*{word}|{word}.*at most 2147483647"):
+                call(n)
