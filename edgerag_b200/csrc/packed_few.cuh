@@ -1,10 +1,13 @@
 // A request's own keys behind a shared prefix, for few rows (bfloat16, heads of 64 and 128, any page size): mma.sync.m16n8k16 on
-// tiles of 16 rows by 16 keys, keys and values fetched by cp.async.  What bounds it is the fetching of keys, so the tensor path matters little
-// here; what matters is that many small blocks are resident and each has its next keys on the way.
+// tiles of 16 rows by 16 keys, keys and values fetched by cp.async.  What bounds it is the fetching of keys (tensor pipe 9 % busy, DRAM 28 %, most
+// waits on global loads), so the tensor path matters little here; what matters is that many small blocks are resident.
 //
 //   attention_own_token_kernel   the rows of one token (up to 16 query heads of a kv head) are one tile; the four warps take 16 keys in turn,
-//                                each with a ring of its own, and are joined at the end.  A request's tokens are done one after the other.
-//   attention_own_rows_kernel    64 rows, (token, head) pairs, 16 for each warp; the four warps share the keys, 32 at a time.
+//                                each with a ring of its own, and are joined at the end.  A warp asks for its next keys when it is done
+//                                with those before (only their page's number is read ahead): the block's other warps and the other blocks
+//                                are what a wait is hidden behind.  A request's tokens are done one after the other.
+//   attention_own_rows_kernel    64 rows, (token, head) pairs, 16 for each warp; the four warps share the keys, 32 at a time, the next three
+//                                times 32 on their way.
 //
 // 256 requests, 32 query heads on 8 of 128: up to 300 own keys behind 4,007 shared ones 66 us in all; 64 own keys each behind 4,096 63 us, by the
 // kernel for many rows 160.
@@ -164,8 +167,9 @@ __device__ __forceinline__ void few_result(const PackedArgs& a, int token, int h
   for (int c = 0; c < C; ++c) dst[lane + 32 * c] = __float2bfloat16_rn(o[c]);
 }
 
-// Two stages: blocks are short (a request's few hundred keys), so four of them on a multiprocessor hide more than a deep ring would (64
-// requests of up to 1,000 own keys behind 16,384: two stages 68 us, three 69, four 75; 256 of up to 300 behind 4,007: 73, 80, 108).
+// Two places, of which one is always empty while a warp multiplies (a place more is a copy under way more); blocks are short (a request's few
+// hundred keys), and three of them (heads of 128) or four on a multiprocessor hide more than a deeper ring, for which fewer fit (64 requests of up to
+// 1,000 own keys behind 16,384: two places 68 us, three 69, four 75; 256 of up to 300 behind 4,007: 73, 80, 108).
 template <int D> struct FewSmem {
   static constexpr int kStages = 2;
   static constexpr uint32_t kTile = 16 * D * 2;                                 // 16 keys or values

@@ -7,9 +7,9 @@
 // Pair i is (i, i + rot_dim / 2) or, with `pairs`, (2i, 2i + 1).  All arithmetic in float, one rounding at the store.
 //
 // The angle.  position * frequency in float loses the angle of far positions: at position 10^6 the fastest pair is off by 0.06 radians.
-// The kernel takes frequencies in turns per position as 64-bit fixed point (`turns`, units of 2^-64 turn), so the integer product with the
-// position, modulo 2^64, is the angle modulo a full turn with an error below position * 2^-65 turns.  Its upper 32 bits are cut into a
-// quadrant and a rest of at most an eighth of a turn, which a float holds to 5e-8 radians.
+// The kernel takes frequencies in turns per position as 64-bit fixed point (`turns`, units of 2^-64 turn, rounded down), so the integer product
+// with the position, modulo 2^64, is the angle modulo a full turn with an error below |position| * 2^-64 turns.  Its upper 32 bits (what is
+// below them is less than 2^-32 turn, 1.5e-9 radians) are cut into a quadrant and a rest of at most an eighth of a turn, which a float holds to 5e-8 radians.
 //
 // Bytes bound it: every entry is read once and written once.  A thread moves 2 V entries that hold whole pairs (V: sixteen bytes of
 // entries), so the lanes of a head exchange nothing but the norm's sum; a token's angles are taken once by the block that works on it.

@@ -86,7 +86,7 @@ class EngineOptions:
     #: launch shapes that do not depend on the batch (decode attention always in splits of 512 keys with
     #: the default grouping of heads; the recurrent mixers walk every token, where a step's longest portion
     #: would otherwise choose between a walk and chunks; portions of differential, latent and 32-bit attention by
-    #: the kernels that take a row the same way in any step): up to 16 single-token rows a request's logits are
+    #: the kernels that take a row the same way in any step, and no prompt from its rows, ``whole_prompts`` or not): up to 16 single-token rows a request's logits are
     #: then the same bits whatever shares its step; off, the kernels follow the batch, which is
     #: faster for small batches, short contexts and portions of prompts
     batch_invariant: bool = False
