@@ -20,7 +20,8 @@
 //   warp 11 (look)      looks over the values of tiles with hidden keys (below)
 //
 // A row's reference maximum moves only when a tile's maximum is 2^8 above it; O is rescaled in TMEM then.  P is a floating-point number, so
-// a reference that is low by eight powers of two costs no precision.
+// a reference that is low by eight powers of two costs no precision.  (References of scores past 2^20: kFarScore in packed.cuh.  The look for
+// them costs 1 to 2 %: prompts of 8,192 tokens of 32 heads of 64 409 -> 415 us, of 32 on 8 of 128 481 -> 483.)
 //
 // A tile's keys are worked on in two halves of 64, each with a place of its own for its scores in TMEM (512 columns: S 2 x 2 x 64, O 2 x D),
 // and P takes the place of the scores it was made of: the next tile's scores of a half are made behind P V of this tile's, while the softmax
@@ -493,7 +494,7 @@ attention_packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
         }
       }
       const int lim_warp = __reduce_min_sync(0xffffffffu, lim);
-      float m_ref = -INFINITY, l = 0.f;
+      float m_ref = -INFINITY, at_ref = -INFINITY, l = 0.f;        // the reference maximum, and the score that it is the scaled one of
 #pragma unroll 1
       for (int half = 0; half < 2 * n; ++half) {                   // 64 keys at a time
         const int i = half >> 1, u = half & 1, key0 = (j0 + i) * BN + 64 * u, g = steps + i;
@@ -512,14 +513,25 @@ attention_packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
           float top[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
           for (int c = 4; c < 64; c += 2) top[(c >> 1) & 3] = max3_nan(top[(c >> 1) & 3], x[c], x[c + 1]);
-          const float m_new = max3_nan(max3_nan(top[0], top[1], top[2]), top[3], top[3]) * a.scale_log2;
-          const bool move = !(m_new <= m_ref + kMoveFrom);
-          if (__any_sync(0xffffffffu, move)) {
+          const float highest = max3_nan(max3_nan(top[0], top[1], top[2]), top[3], top[3]), m_new = highest * a.scale_log2;
+          float minus = m_ref;
+          if (__any_sync(0xffffffffu, !(m_new <= m_ref + kMoveFrom) || fabsf(m_new) > kFarScore)) {
+            const bool move = !(m_new <= m_ref + kMoveFrom) || (far_score(m_new) && highest > at_ref);
             // (0 for the first keys.  A row with a score that is no number, or infinite, becomes NaN as a whole.)
-            const float alpha = move ? fast_exp2(m_ref - m_new) : 1.f;
-            if (move) m_ref = m_new < INFINITY ? m_new : NAN;
+            const float alpha = move ? fast_exp2(far_score(m_new) || far_score(m_ref) ? (at_ref - highest) * a.scale_log2 : m_ref - m_new) : 1.f;
+            if (move) {
+              m_ref = m_new < INFINITY ? m_new : NAN;
+              at_ref = highest;
+            }
+            const bool far = far_score(m_ref);
+            if (__any_sync(0xffffffffu, far)) {
+              const float from = far ? at_ref : 0.f;
+#pragma unroll
+              for (int c = 0; c < 64; ++c) x[c] -= from;
+            }
+            minus = far ? 0.f : m_ref;
             l *= alpha;
-            if (half > 0) {
+            if (half > 0 && __any_sync(0xffffffffu, move)) {
               if (!wait(C::kPv + 2 * (u ^ 1) + t, u ? g : g - 1)) break;      // P V of the half before
               fence_after_sync();
 #pragma unroll 1
@@ -534,7 +546,7 @@ attention_packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gr
               tmem_st_wait();
             }
           }
-          const Two scale2(a.scale_log2), minus2(m_ref == -INFINITY ? 0.f : -m_ref);
+          const Two scale2(a.scale_log2), minus2(minus == -INFINITY ? 0.f : -minus);
           Two sum2[2] = {Two(0.f), Two(0.f)};
           uint32_t packed[32];
 #pragma unroll

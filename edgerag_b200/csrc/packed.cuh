@@ -29,6 +29,12 @@ constexpr int kPrompt = 0, kPrefix = 1, kOwn = 2;
 // Codes of the status word beside those of waits: a page that lies outside the pool, sequences that do not lie inside the rows.
 constexpr int kBadPage = 9000001, kBadStarts = 9000002;
 
+// Scaled scores (log2 domain) from here on: half a step of a float is a sixteenth at 2^20, and past 2^30 more exponents than a float has, so that a
+// weight made from a scaled score and its row's rounded maximum could be infinite, or all of a row's be zero.  A row whose reference maximum lies beyond takes
+// its scores' distances to the reference's score before they are scaled: exact for those that matter, and the highest one's weight is 1.
+constexpr float kFarScore = 1048576.f;
+__device__ __forceinline__ bool far_score(float m) { return fabsf(m) > kFarScore && m > -INFINITY; }
+
 struct PackedArgs {
   const elem_t* q;
   elem_t* out;

@@ -30,7 +30,7 @@ template <int D> __device__ __forceinline__ uint32_t few_at(int r, int c) { retu
 // 16 rows of one warp: rows g = lane / 4 and g + 8, the running maximum (log2 domain), sum and result of each.
 template <int D> struct FewRows {
   uint32_t q[D / 16][4];
-  float m[2], l[2], o[D / 8][4];
+  float m[2], at[2], l[2], o[D / 8][4];            // at: the score that m is the scaled one of
 
   __device__ __forceinline__ void start(const elem_t* row0, const elem_t* row1) {         // the two rows' queries, or null
     const int q2 = (threadIdx.x & 3) * 2;
@@ -42,7 +42,7 @@ template <int D> struct FewRows {
       q[k][2] = row0 ? __ldcg(reinterpret_cast<const unsigned*>(row0 + c + 8)) : 0u;
       q[k][3] = row1 ? __ldcg(reinterpret_cast<const unsigned*>(row1 + c + 8)) : 0u;
     }
-    m[0] = m[1] = -INFINITY;
+    m[0] = m[1] = at[0] = at[1] = -INFINITY;
     l[0] = l[1] = 0.f;
 #pragma unroll
     for (int d = 0; d < D / 8; ++d) o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.f;
@@ -74,20 +74,33 @@ template <int D> struct FewRows {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
-      top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2)) * scale_log2;
+      top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
     }
     // (the reference maximum moves as in the kernel for many rows: from 2^8 above it on)
-    const bool move0 = top[0] > m[0] + 8.f, move1 = top[1] > m[1] + 8.f;
-    if (__any_sync(0xffffffffu, move0 || move1)) {
-      const float a0 = move0 ? fast_exp2(m[0] - top[0]) : 1.f, a1 = move1 ? fast_exp2(m[1] - top[1]) : 1.f;
-      if (move0) m[0] = top[0];
-      if (move1) m[1] = top[1];
+    const float n0 = top[0] * scale_log2, n1 = top[1] * scale_log2;
+    float b0 = m[0], b1 = m[1];
+    if (__any_sync(0xffffffffu, n0 > m[0] + 8.f || n1 > m[1] + 8.f || fabsf(n0) > kFarScore || fabsf(n1) > kFarScore)) {
+      const bool move0 = n0 > m[0] + 8.f || (far_score(n0) && top[0] > at[0]), move1 = n1 > m[1] + 8.f || (far_score(n1) && top[1] > at[1]);
+      const float a0 = move0 ? fast_exp2(far_score(n0) || far_score(m[0]) ? (at[0] - top[0]) * scale_log2 : m[0] - n0) : 1.f;
+      const float a1 = move1 ? fast_exp2(far_score(n1) || far_score(m[1]) ? (at[1] - top[1]) * scale_log2 : m[1] - n1) : 1.f;
+      if (move0) { m[0] = n0; at[0] = top[0]; }
+      if (move1) { m[1] = n1; at[1] = top[1]; }
+      const bool far0 = far_score(m[0]), far1 = far_score(m[1]);
+      if (__any_sync(0xffffffffu, far0 || far1)) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[t][e] -= e < 2 ? (far0 ? at[0] : 0.f) : (far1 ? at[1] : 0.f);
+      }
+      b0 = far0 ? 0.f : m[0];
+      b1 = far1 ? 0.f : m[1];
       l[0] *= a0;
       l[1] *= a1;
 #pragma unroll
       for (int d = 0; d < D / 8; ++d) { o[d][0] *= a0; o[d][1] *= a0; o[d][2] *= a1; o[d][3] *= a1; }
     }
-    const float b0 = m[0] == -INFINITY ? 0.f : m[0], b1 = m[1] == -INFINITY ? 0.f : m[1];
+    b0 = b0 == -INFINITY ? 0.f : b0;
+    b1 = b1 == -INFINITY ? 0.f : b1;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       const float x0 = fast_exp2(fmaf(s[t][0], scale_log2, -b0)), x1 = fast_exp2(fmaf(s[t][1], scale_log2, -b0));
