@@ -32,10 +32,10 @@
 // nobody sees become zeros, and an infinity or NaN that only some rows see becomes zero and is added to exactly those rows at the end.
 //
 // What bounds it: a half step's chain, scores -> softmax -> P V, that two query tiles only partly hide from each other (polynomial exponentials,
-// sixteen softmax warps and smaller chunks of P made it slower), and the tail of uneven pieces.  8,192 tokens, 32 query heads on 8 of 128: 480 us,
-// 1.15 PFLOP/s, 0.69 of a library product's rate (550 us and 0.60 called without a pause, under the power limit; in steps as they were built: a block
-// for each piece 700, one issuing warp 583, one tile of 128 keys at a time 545, as it is 489; CUDA cores 20,650); of heads of 64, 32 of them, 405 us.
-// 23 prompts of up to 2,001 tokens, 32 heads of 64: 150 us.  16,384 keys of 8 heads of 128 before 1 row 27 us (2.5 TB/s), 8 30, 64 44, with the
+// sixteen softmax warps and smaller chunks of P made it slower), and the tail of uneven pieces.  8,192 tokens, 32 query heads on 8 of 128: 483 us,
+// 1.14 PFLOP/s, 0.69 of a library product's rate (550 us and 0.60 called without a pause, under the power limit; in steps as they were built: a block
+// for each piece 700, one issuing warp 583, one tile of 128 keys at a time 545, as it is 489; CUDA cores 20,650); of heads of 64, 32 of them, 415 us.
+// 23 prompts of up to 2,001 tokens, 32 heads of 64: 153 us.  16,384 keys of 8 heads of 128 before 1 row 27 us (2.5 TB/s), 8 30, 64 45, with the
 // pieces' records written and joined.
 //
 // Every wait is bounded: a thread that gives up raises a block-wide flag, every other wait of the block then ends too, the block records a

@@ -9,7 +9,7 @@
 //   attention_own_rows_kernel    64 rows, (token, head) pairs, 16 for each warp; the four warps share the keys, 32 at a time, the next three
 //                                times 32 on their way.
 //
-// 256 requests, 32 query heads on 8 of 128: up to 300 own keys behind 4,007 shared ones 66 us in all; 64 own keys each behind 4,096 63 us, by the
+// 256 requests, 32 query heads on 8 of 128: up to 300 own keys behind 4,007 shared ones 68 us in all; 64 own keys each behind 4,096 63 us, by the
 // kernel for many rows 160.
 //
 // Where the prefix's records are all that is left to join (`final`) the block does that too and writes the result.  It may run while the

@@ -36,9 +36,9 @@ tensor ``vmix``).
 With positions scaled for long contexts (``rope_scaled``) the norm per head, the rotation and the cache write are one kernel
 (``kernels.rotary_append``).  ``whole_prompts``: where every portion of a step is its prompt's beginning, keys and values are taken from the step's
 rows instead of the cache (``kernels.attention_prompt``: tensor cores for heads of 64 and 128); positions then have to be scaled ones or none,
-since only those leave the rows' keys as the cache has them (rows | pages, in microseconds: bfloat16, 32 heads of 64, prompts of 48 tokens 7.8 | 7.1, 512
-13.7 | 14.7, 8,192 400 | 440, 23 of up to 2,001 148 | 198; 9 on 3 of 64, 333 tokens 13.2 | 12.2; 32 on 8 of 128, 512 tokens 17 | 629; float32, 9 on 3 of 64, 20
-tokens 7.6 | 4.9, 333 27.9 | 26.2, 1,000 103 | 109).  A call that reads the cache another call wrote takes its keys from there, and
+since only those leave the rows' keys as the cache has them (rows | pages, in microseconds: bfloat16, 32 heads of 64, prompts of 48 tokens 7.9 | 7.1, 512
+14.3 | 14.8, 8,192 409 | 440, 23 of up to 2,001 151 | 198; 9 on 3 of 64, 333 tokens 13.2 | 12.3; 32 on 8 of 128, 512 tokens 17 | 629; float32, 9 on 3 of 64, 20
+tokens 7.6 | 4.9, 333 27.8 | 26.1, 1,000 103 | 109).  A call that reads the cache another call wrote takes its keys from there, and
 with ``EngineOptions.batch_invariant`` every portion does: another request's portion with a past would otherwise change a prompt's kernel.
 
 Heads whose sizes differ or are no multiple of 8 are stored padded with zeros to one size ``D``:
